@@ -388,6 +388,61 @@ int b200q_dequantize(int type, int elem, const void* w, void* out, long long nro
 int b200q_get_rows(int type, int elem, const void* w, const int32_t* ids, void* out, long long n_ids, int K, long long nrows_w,
                    void* stream);
 
+/* Int8 rows with a scale each: weights with one per output channel, activations with one per token.
+ *   s = max|x| / 127 (rounded to f32), q = the integer next to x / s, ties to the even one; a row with an infinity or a
+ * NaN in it has a NaN for a scale and zeros for integers. q rows are ldq bytes apart (a multiple of 16, >= k, q 16-byte
+ * aligned); the bytes from k to the next multiple of 16 are written as zeros, and every product below relies on that.
+ * x rows are ldx values of element type `elem` apart. */
+int b200q_int8_quantize(int elem, const void* x, long long ldx, void* q, long long ldq, float* scales, long long rows, int k,
+                        void* stream);
+int b200q_int8_dequantize(int elem, const void* q, long long ldq, const float* scales, void* out, long long rows, int k, void* stream);
+
+/* y[r][i] = (sum_k xq[r][k] wq[e][i][k]) * xs[r] * ws[e][i], the sum an exact integer (k at most 131072), the rest in f32,
+ * y of element type `elem`. Several matrices wq [experts][n] and scales ws [experts][n]: rows offsets[e] .. offsets[e + 1]
+ * belong to matrix e (offsets: experts + 1 device ints that do not fall, the last at most `rows`); rows of y behind
+ * offsets[experts] are left as they are. One matrix with all rows: experts 1, offsets null. */
+int b200q_int8_gemm(int elem, const void* xq, const float* xs, const void* wq, const float* ws, void* y, int rows, int n, int k,
+                    long long ldx, long long ldw, long long ldy, const int* offsets, int experts, void* stream);
+
+/* y[m][ldy] = x[m][ldx] . W^T for int8 weights: b200q_int8_quantize into the workspace (128-byte aligned,
+ * b200q_int8_matmul_workspace_bytes bytes, nothing kept in it between calls), then the product. */
+long long b200q_int8_matmul_workspace_bytes(int m, int k);
+int b200q_int8_matmul(int elem, const void* x, const void* wq, const float* ws, void* y, int m, int n, int k, long long ldx,
+                      long long ldw, long long ldy, void* workspace, long long workspace_bytes, void* stream);
+
+/* Slots sorted by expert: ids are `slots` expert numbers of id_bytes 4 or 8. position[slot] = its row, -1 where the id is
+ * no expert's; order[row] = its slot, -1 behind the last row; rows of expert e are offsets[e] .. offsets[e + 1]. Slots of
+ * one expert keep their order. */
+int b200q_route_sort(const void* ids, int id_bytes, int slots, int experts, int* order, int* offsets, int* position, void* stream);
+
+/* Rows [tokens * topk][h] of the experts from tokens x [tokens][ldx], and back. position and offsets as b200q_route_sort
+ * leaves them (slot = token * topk + j).
+ *  dispatch:     rows[position[t, j]] = x[t]; rows behind the last are zeroed.
+ *  combine:      out[t] = sum_j weights[t, j] * rows[position[t, j]] in f32, slots without a row left out; weights null: 1
+ *                each (the gradient of dispatch). Never reads a row that no slot has.
+ *  combine_grad: grad_rows[position[t, j]] = weights[t, j] * grad_out[t] (rows behind the last zeroed) and
+ *                grad_weights[t, j] = <grad_out[t], rows[position[t, j]]>, 0 for slots without a row; either may be null. */
+int b200q_route_dispatch(int elem, const void* x, long long ldx, const int* position, const int* offsets, int experts, void* rows,
+                         int tokens, int topk, int h, void* stream);
+int b200q_route_combine(int elem_in, int elem_out, const void* rows, long long ldr, const int* position, const float* weights,
+                        void* out, int tokens, int topk, int h, void* stream);
+int b200q_route_combine_grad(int elem_grad, int elem, const void* grad_out, long long ldg, const void* rows, long long ldr,
+                             const int* position, const int* offsets, int experts, const float* weights, void* grad_rows,
+                             float* grad_weights, int tokens, int topk, int h, void* stream);
+
+/* A layer of gated experts on int8 weights: out[t] = sum_j weights[t, j] * down_e(act(gate_e(x[t])) * up_e(x[t])) with
+ * e = ids[t, j] (a slot whose id is no expert's counts as nothing). x and out of element type `elem`; the hidden values
+ * are held in that type and become int8 rows again, the experts' outputs are held in f32.
+ *  gate_up: [experts][2 * p][hidden] with p = ffn rounded up to 8, 8 rows of gate and 8 of up in turn (the rows that fill
+ *  up hold zeros); down: [experts][hidden][ffn]; both with rows padded to 16 bytes, and scales [experts][2 * p] / [hidden].
+ *  activation: 0 SiLU, 1 GELU (tanh), 2 ReLU, 3 GELU (erf), 4 sigmoid.
+ *  workspace: 128-byte aligned, nothing kept in it between calls. */
+long long b200q_int8_experts_workspace_bytes(int elem, int tokens, int topk, int experts, int hidden, int ffn);
+int b200q_int8_experts(int elem, int activation, const void* x, long long ldx, const void* ids, int id_bytes, const float* weights,
+                       const void* gate_up, const float* gate_up_scales, const void* down, const float* down_scales, void* out,
+                       int tokens, int experts, int topk, int hidden, int ffn, void* workspace, long long workspace_bytes,
+                       void* stream);
+
 /* out = {staged kernel?, grid, dynamic smem bytes, stages, rows per stage, warps per row, stage bytes, rows per unit of
  *        the CTAs' row partition (the 16-byte alignment unit, or a whole stage for short launches), item slots per lane,
  *        register-resident slots} */

@@ -8,4 +8,6 @@ from . import kernel_library  # noqa: F401
 from .kernel_library import KernelLibraryError, library  # noqa: F401
 from .dtypes import GgmlDType  # noqa: F401
 from .qmatmul import GgufMatMul, QMatMul, QTensor  # noqa: F401
+from .int8 import Int8Experts, Int8MatMul, Int8Tensor  # noqa: F401
+from .routing import TokenRouting  # noqa: F401
 from . import gguf_file  # noqa: F401

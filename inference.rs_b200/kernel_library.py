@@ -80,6 +80,17 @@ SYMBOLS.update({
     "b200q_dequantize": ([_i32, _i32, _vp, _vp, _i64, _i32, _vp], _i32),
     "b200q_get_rows": ([_i32, _i32, _vp, _vp, _vp, _i64, _i32, _i64, _vp], _i32),
     "b200q_clear_weight_successors": ([], _i32),
+    "b200q_int8_quantize": ([_i32, _vp, _i64, _vp, _i64, _vp, _i64, _i32, _vp], _i32),
+    "b200q_int8_dequantize": ([_i32, _vp, _i64, _vp, _vp, _i64, _i32, _vp], _i32),
+    "b200q_int8_gemm": ([_i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64, _i64, _vp, _i32, _vp], _i32),
+    "b200q_int8_matmul_workspace_bytes": ([_i32, _i32], _i64),
+    "b200q_int8_matmul": ([_i32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _i64, _i64, _vp, _i64, _vp], _i32),
+    "b200q_route_sort": ([_vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp], _i32),
+    "b200q_route_dispatch": ([_i32, _vp, _i64, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _vp], _i32),
+    "b200q_route_combine": ([_i32, _i32, _vp, _i64, _vp, _vp, _vp, _i32, _i32, _i32, _vp], _i32),
+    "b200q_route_combine_grad": ([_i32, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp], _i32),
+    "b200q_int8_experts_workspace_bytes": ([_i32] * 6, _i64),
+    "b200q_int8_experts": ([_i32, _i32, _vp, _i64, _vp, _i32] + [_vp] * 6 + [_i32] * 5 + [_vp, _i64, _vp], _i32),
 })
 DATA_SYMBOLS = ["inference_kernel_build_id"]
 

@@ -362,6 +362,233 @@ def gemv_tc(dtype: GgmlDType, w: torch.Tensor, x: torch.Tensor, n: int, out: tor
     return y
 
 
+# ---- int8 rows with a scale each, and the routing of tokens to experts ----
+# These take tensors of any device: the launch goes to the current stream of the tensors' own.
+
+INT8_ROW_ALIGN = 16  # int8 rows start on such boundaries; what lies between k and the next one is zero
+
+
+def _one_device(*tensors: torch.Tensor) -> torch.device:
+    for t in tensors:
+        if not t.is_cuda:
+            raise ValueError("expected a CUDA tensor")
+        if t.device != tensors[0].device:
+            raise ValueError(f"tensors on {tensors[0].device} and {t.device}")
+    return tensors[0].device
+
+
+def _rows2d(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int]:
+    """A matrix whose rows have unit stride and do not overlap, and the distance between them; copied where it is not one."""
+    if t.dim() != 2:
+        raise ValueError(f"{what}: expected a matrix, got {tuple(t.shape)}")
+    if t.numel() and t.shape[0] > 1 and t.shape[1] > 1 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
+        return t, t.stride(0)
+    return t.contiguous(), t.shape[1]
+
+
+def _check_vector(t: torch.Tensor, dtype: torch.dtype, numel: int, what: str) -> None:
+    if t.dtype != dtype:
+        raise TypeError(f"{what} must be {dtype}, not {t.dtype}")
+    if t.numel() != numel or not t.is_contiguous():
+        raise ValueError(f"{what}: expected {numel} contiguous values, got {tuple(t.shape)}")
+
+
+def _check_int8_rows(q: torch.Tensor, k: int, what: str) -> None:
+    if q.dtype != torch.int8:
+        raise TypeError(f"{what} must be int8, not {q.dtype}")
+    if q.dim() != 2 or not q.is_contiguous() or q.shape[1] != pad(k, INT8_ROW_ALIGN) or q.data_ptr() % 16:
+        raise ValueError(f"{what}: expected contiguous rows of {pad(k, INT8_ROW_ALIGN)} bytes on 16-byte boundaries, got {tuple(q.shape)}")
+
+
+def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """`b200q_int8_quantize`: rows x [m, k] (f32, f16 or bf16) -> int8 [m, k padded to 16] and a f32 scale per row, max|row| / 127.
+    A row with an infinity or a NaN in it gets a NaN for a scale."""
+    elem = elem_of(x.dtype)
+    dev = _one_device(x)
+    x, ldx = _rows2d(x, "int8_quantize")
+    m, k = x.shape
+    q = torch.empty((m, pad(k, INT8_ROW_ALIGN)), dtype=torch.int8, device=dev)
+    scales = torch.empty(m, dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        kl.check(kl.library().b200q_int8_quantize(elem, x.data_ptr(), ldx, q.data_ptr(), q.shape[1], scales.data_ptr(), m, k, _stream()),
+                 "b200q_int8_quantize")
+    return q, scales
+
+
+def int8_dequantize(q: torch.Tensor, scales: torch.Tensor, k: int, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """`b200q_int8_dequantize`: int8 rows and their scales -> the values [m, k] they stand for."""
+    elem = elem_of(out_dtype)
+    dev = _one_device(q, scales)
+    _check_int8_rows(q, k, "int8 rows")
+    _check_vector(scales, torch.float32, q.shape[0], "scales")
+    out = torch.empty((q.shape[0], k), dtype=out_dtype, device=dev)
+    with torch.cuda.device(dev):
+        kl.check(kl.library().b200q_int8_dequantize(elem, q.data_ptr(), q.shape[1], scales.data_ptr(), out.data_ptr(), q.shape[0], k, _stream()),
+                 "b200q_int8_dequantize")
+    return out
+
+
+def int8_gemm(xq: torch.Tensor, x_scales: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor, k: int, out_dtype: torch.dtype,
+              offsets: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """`b200q_int8_gemm`: rows xq [m, kp] of int8 times wq [n, kp], scaled by token and channel -> [m, n]. With wq [experts, n, kp],
+    w_scales [experts, n] and int32 offsets [experts + 1] rows offsets[e]..offsets[e + 1] meet matrix e; the rows behind the last
+    expert's are not written."""
+    elem = elem_of(out_dtype)
+    dev = _one_device(xq, x_scales, wq, w_scales, *(t for t in (offsets, out) if t is not None))
+    experts = wq.shape[0] if wq.dim() == 3 else 1
+    n = wq.shape[-2]
+    _check_int8_rows(xq, k, "activations")
+    _check_int8_rows(wq.reshape(-1, wq.shape[-1]) if wq.is_contiguous() else wq, k, "weights")
+    _check_vector(x_scales, torch.float32, xq.shape[0], "token scales")
+    _check_vector(w_scales, torch.float32, experts * n, "channel scales")
+    if wq.dim() == 3 and offsets is None:
+        raise ValueError("several matrices need offsets")
+    if offsets is not None:
+        _check_vector(offsets, torch.int32, experts + 1, "offsets")
+    y = torch.empty((xq.shape[0], n), dtype=out_dtype, device=dev) if out is None else out
+    if y.dtype != out_dtype or y.shape != (xq.shape[0], n) or not y.is_contiguous():
+        raise ValueError(f"out: expected a contiguous {out_dtype} matrix of {(xq.shape[0], n)}")
+    with torch.cuda.device(dev):
+        kl.check(kl.library().b200q_int8_gemm(elem, xq.data_ptr(), x_scales.data_ptr(), wq.data_ptr(), w_scales.data_ptr(), y.data_ptr(),
+                                              xq.shape[0], n, k, xq.shape[1], wq.shape[-1], n, offsets.data_ptr() if offsets is not None else None,
+                                              experts, _stream()), "b200q_int8_gemm")
+    return y
+
+
+def int8_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor) -> torch.Tensor:
+    """`b200q_int8_matmul`: x [m, k] (f32, f16 or bf16; rows may be strided) becomes int8 rows, times wq [n, kp] -> [m, n] of x's
+    type."""
+    elem = elem_of(x.dtype)
+    dev = _one_device(x, wq, w_scales)
+    x, ldx = _rows2d(x, "int8_matmul")
+    m, k = x.shape
+    _check_int8_rows(wq, k, "weights")
+    n = wq.shape[0]
+    _check_vector(w_scales, torch.float32, n, "channel scales")
+    y = torch.empty((m, n), dtype=x.dtype, device=dev)
+    lib = kl.library()
+    nbytes = int(lib.b200q_int8_matmul_workspace_bytes(m, k))
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        kl.check(lib.b200q_int8_matmul(elem, x.data_ptr(), wq.data_ptr(), w_scales.data_ptr(), y.data_ptr(), m, n, k, ldx, wq.shape[1], n,
+                                       ws.data_ptr(), nbytes, _stream()), "b200q_int8_matmul")
+    return y
+
+
+def route_sort(ids: torch.Tensor, experts: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """`b200q_route_sort`: expert ids (int32 or int64, any shape; others than 0..experts - 1 mean none) -> order [slots], offsets
+    [experts + 1], position [*ids.shape], all int32: row r is slot order[r] (-1 behind the last row), expert e's rows are
+    offsets[e]..offsets[e + 1], slot s is row position[s] (-1: none)."""
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"expert ids must be int32 or int64, not {ids.dtype}")
+    dev = _one_device(ids)
+    ids = ids.contiguous()
+    order = torch.empty(ids.numel(), dtype=torch.int32, device=dev)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev) if experts >= 0 else torch.empty(0, dtype=torch.int32, device=dev)
+    position = torch.empty(ids.shape, dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        kl.check(kl.library().b200q_route_sort(ids.data_ptr(), ids.element_size(), ids.numel(), experts, order.data_ptr(), offsets.data_ptr(),
+                                               position.data_ptr(), _stream()), "b200q_route_sort")
+    return order, offsets, position
+
+
+def _check_position(position: torch.Tensor, tokens: int | None = None) -> None:
+    if position.dtype != torch.int32:
+        raise TypeError(f"positions must be int32, not {position.dtype}")
+    if position.dim() != 2 or not position.is_contiguous() or (tokens is not None and position.shape[0] != tokens):
+        raise ValueError(f"positions: expected a contiguous [tokens, slots] matrix, got {tuple(position.shape)}")
+
+
+def route_dispatch(x: torch.Tensor, position: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """`b200q_route_dispatch`: x [tokens, h] -> rows [tokens * slots, h] in the order of the experts; rows behind the last are zeros."""
+    elem = elem_of(x.dtype)
+    dev = _one_device(x, position, offsets)
+    x, ldx = _rows2d(x, "route_dispatch")
+    tokens, h = x.shape
+    _check_position(position, tokens)
+    _check_vector(offsets, torch.int32, offsets.numel(), "offsets")
+    topk = position.shape[1]
+    rows = torch.empty((tokens * topk, h), dtype=x.dtype, device=dev)
+    with torch.cuda.device(dev):
+        kl.check(kl.library().b200q_route_dispatch(elem, x.data_ptr(), ldx, position.data_ptr(), offsets.data_ptr(), offsets.numel() - 1,
+                                                   rows.data_ptr(), tokens, topk, h, _stream()), "b200q_route_dispatch")
+    return rows
+
+
+def route_combine(rows: torch.Tensor, position: torch.Tensor, weights: torch.Tensor | None, out_dtype: torch.dtype) -> torch.Tensor:
+    """`b200q_route_combine`: rows [tokens * slots, h] back to [tokens, h], each token the sum of its rows times its weights (f32
+    [tokens, slots]; None: 1 each), in f32 and in slot order."""
+    elem_in, elem_out = elem_of(rows.dtype), elem_of(out_dtype)
+    dev = _one_device(rows, position, *(() if weights is None else (weights,)))
+    rows, ldr = _rows2d(rows, "route_combine")
+    _check_position(position)
+    tokens, topk = position.shape
+    if rows.shape[0] != tokens * topk:
+        raise ValueError(f"route_combine: {rows.shape[0]} rows for {tokens} x {topk} slots")
+    if weights is not None:
+        _check_vector(weights, torch.float32, tokens * topk, "weights")
+    out = torch.empty((tokens, rows.shape[1]), dtype=out_dtype, device=dev)
+    with torch.cuda.device(dev):
+        kl.check(kl.library().b200q_route_combine(elem_in, elem_out, rows.data_ptr(), ldr, position.data_ptr(),
+                                                  None if weights is None else weights.data_ptr(), out.data_ptr(), tokens, topk, rows.shape[1],
+                                                  _stream()), "b200q_route_combine")
+    return out
+
+
+def route_combine_grad(grad_out: torch.Tensor, rows: torch.Tensor, position: torch.Tensor, offsets: torch.Tensor, weights: torch.Tensor,
+                       need_rows: bool = True, need_weights: bool = True) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """`b200q_route_combine_grad`: the gradients of `route_combine` towards its rows (in their type) and its weights (f32)."""
+    elem_g, elem = elem_of(grad_out.dtype), elem_of(rows.dtype)
+    dev = _one_device(grad_out, rows, position, offsets, weights)
+    grad_out, ldg = _rows2d(grad_out, "route_combine_grad")
+    rows, ldr = _rows2d(rows, "route_combine_grad")
+    _check_position(position, grad_out.shape[0])
+    _check_vector(offsets, torch.int32, offsets.numel(), "offsets")
+    tokens, topk = position.shape
+    _check_vector(weights, torch.float32, tokens * topk, "weights")
+    if tuple(rows.shape) != (tokens * topk, grad_out.shape[1]):
+        raise ValueError(f"route_combine_grad: rows {tuple(rows.shape)} and gradient {tuple(grad_out.shape)} for {tokens} x {topk} slots")
+    grad_rows = torch.empty_like(rows, memory_format=torch.contiguous_format) if need_rows else None
+    grad_weights = torch.empty((tokens, topk), dtype=torch.float32, device=dev) if need_weights else None
+    with torch.cuda.device(dev):
+        kl.check(kl.library().b200q_route_combine_grad(elem_g, elem, grad_out.data_ptr(), ldg, rows.data_ptr(), ldr, position.data_ptr(),
+                                                       offsets.data_ptr(), offsets.numel() - 1, weights.data_ptr(),
+                                                       None if grad_rows is None else grad_rows.data_ptr(),
+                                                       None if grad_weights is None else grad_weights.data_ptr(), tokens, topk, grad_out.shape[1],
+                                                       _stream()), "b200q_route_combine_grad")
+    return grad_rows, grad_weights
+
+
+def int8_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate_up: torch.Tensor, gate_up_scales: torch.Tensor,
+                 down: torch.Tensor, down_scales: torch.Tensor, ffn: int, activation: str = "silu") -> torch.Tensor:
+    """`b200q_int8_experts`: x [tokens, h] through the experts that ids [tokens, slots] names, weighted (f32). gate_up as
+    `Int8Experts` lays it out."""
+    elem = elem_of(x.dtype)
+    dev = _one_device(x, ids, weights, gate_up, gate_up_scales, down, down_scales)
+    x, ldx = _rows2d(x, "int8_experts")
+    tokens, hidden = x.shape
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"expert ids must be int32 or int64, not {ids.dtype}")
+    if ids.dim() != 2 or ids.shape[0] != tokens or not ids.is_contiguous():
+        raise ValueError(f"ids: expected a contiguous [{tokens}, slots] matrix, got {tuple(ids.shape)}")
+    experts, topk, p = gate_up.shape[0], ids.shape[1], pad(ffn, 8)
+    _check_vector(weights, torch.float32, tokens * topk, "weights")
+    for t, shape, what in ((gate_up, (experts, 2 * p, pad(hidden, 16)), "gate_up"), (down, (experts, hidden, pad(ffn, 16)), "down")):
+        if tuple(t.shape) != shape or t.dtype != torch.int8 or not t.is_contiguous():
+            raise ValueError(f"{what}: expected contiguous int8 {shape}, got {t.dtype} {tuple(t.shape)}")
+    _check_vector(gate_up_scales, torch.float32, experts * 2 * p, "gate_up scales")
+    _check_vector(down_scales, torch.float32, experts * hidden, "down scales")
+    out = torch.empty((tokens, hidden), dtype=x.dtype, device=dev)
+    lib = kl.library()
+    nbytes = int(lib.b200q_int8_experts_workspace_bytes(elem, tokens, topk, experts, hidden, ffn))
+    ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        kl.check(lib.b200q_int8_experts(elem, GLU_ACTIVATIONS[activation], x.data_ptr(), ldx, ids.data_ptr(), ids.element_size(), weights.data_ptr(),
+                                        gate_up.data_ptr(), gate_up_scales.data_ptr(), down.data_ptr(), down_scales.data_ptr(), out.data_ptr(),
+                                        tokens, experts, topk, hidden, ffn, ws.data_ptr(), nbytes, _stream()), "b200q_int8_experts")
+    return out
+
+
 def set_weight_successor(w: torch.Tensor, next_w: torch.Tensor | None, next_dtype: GgmlDType | None = None, next_k: int = 0,
                          next_n: int = 0) -> None:
     """`b200q_set_weight_successor`: the decode launch after the one on `w` will read `next_w` [next_n, next_k]; every
