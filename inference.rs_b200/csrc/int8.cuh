@@ -62,6 +62,9 @@ cudaError_t int8_quantize_rows(int elem, const void* x, long long ldx, int8_t* q
 cudaError_t int8_dequantize_rows(int elem, const int8_t* q, long long ldq, const float* scales, void* out, long long rows, int k, cudaStream_t s);
 // int8_rows.cu
 cudaError_t int8_product_rows(int elem, const Int8Product& p, cudaStream_t s, bool dependent);
+// int8_pair.cu
+bool int8_pair_pays(const Int8Product& p);
+int int8_product_pair(int elem, const Int8Product& p, cudaStream_t s, bool dependent);
 // token_routing.cu
 cudaError_t route_sort(const void* ids, bool wide, int slots, int experts, int* order, int* offsets, int* position, cudaStream_t s);
 cudaError_t route_dispatch(int elem, const void* x, long long ldx, const int* position, const int* valid, void* rows, int tokens, int topk, int h,

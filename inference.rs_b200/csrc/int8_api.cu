@@ -27,7 +27,10 @@ static int check_routing(long long tokens, int topk, int experts) {
     return B200Q_OK;
 }
 
-static cudaError_t int8_product(int elem, const Int8Product& p, cudaStream_t s, bool dependent) { return int8_product_rows(elem, p, s, dependent); }
+static int int8_product(int elem, const Int8Product& p, cudaStream_t s, bool dependent) {
+    if (int8_pair_pays(p)) return int8_product_pair(elem, p, s, dependent);
+    return cuda_result(int8_product_rows(elem, p, s, dependent));
+}
 
 // What the experts' layer keeps between its launches, one region after the other, each on a 256-byte boundary.
 struct ExpertsWorkspace {
@@ -93,7 +96,7 @@ int b200q_int8_gemm(int elem, const void* xq, const float* xs, const void* wq, c
     if (!elem_ok(elem)) return set_error(B200Q_ERR_UNSUPPORTED, "outputs are f32, f16 or bf16");
     if (const int rc = check_k(k)) return rc;
     if (rows < 0 || n < 0 || ldy < n) return set_error(B200Q_ERR_INVALID, "bad shape");
-    if (experts < 1 || experts > INT8_MAX_EXPERTS || (long long)experts * n > INT_MAX) return set_error(B200Q_ERR_UNSUPPORTED, "1 to 1024 matrices of 2^31 rows in all");
+    if (experts < 1 || experts > INT8_MAX_EXPERTS || (long long)experts * n > INT_MAX - 512) return set_error(B200Q_ERR_UNSUPPORTED, "1 to 1024 matrices of 2^31 rows in all");
     if (experts > 1 && !offsets) return set_error(B200Q_ERR_INVALID, "several matrices need offsets");
     if (rows == 0 || n == 0) return B200Q_OK;
     if (!xq || !xs || !wq || !ws || !y) return set_error(B200Q_ERR_INVALID, "null pointer");
@@ -102,7 +105,7 @@ int b200q_int8_gemm(int elem, const void* xq, const float* xs, const void* wq, c
     if (const int rc = check_int8_rows(wq, ldw, k, align)) return rc;
     if (ldx > INT_MAX || ldw > INT_MAX) return set_error(B200Q_ERR_INVALID, "rows too far apart");
     const Int8Product p{static_cast<const int8_t*>(xq), xs, static_cast<const int8_t*>(wq), ws, y, offsets, rows, n, k, (int)ldx, (int)ldw, experts, INT8_ACT_NONE, n, ldy, status_ptr()};
-    return cuda_result(int8_product(elem, p, (cudaStream_t)stream, false));
+    return int8_product(elem, p, (cudaStream_t)stream, false);
 }
 
 long long b200q_int8_matmul_workspace_bytes(int m, int k) {
@@ -128,7 +131,7 @@ int b200q_int8_matmul(int elem, const void* x, const void* wq, const float* ws, 
     const cudaError_t e = int8_quantize_rows(elem, x, ldx, xq, kp, xs, m, k, nullptr, 1, nullptr, s, false);
     if (e != cudaSuccess) return cuda_result(e);
     const Int8Product p{xq, xs, static_cast<const int8_t*>(wq), ws, y, nullptr, m, n, k, (int)kp, (int)ldw, 1, INT8_ACT_NONE, n, ldy, status_ptr()};
-    return cuda_result(int8_product(elem, p, s, true));
+    return int8_product(elem, p, s, true);
 }
 
 int b200q_route_sort(const void* ids, int id_bytes, int slots, int experts, int* order, int* offsets, int* position, void* stream) {
@@ -185,7 +188,7 @@ int b200q_int8_experts(int elem, int activation, const void* x, long long ldx, c
     if (const int rc = check_k(ffn)) return rc;
     if (ldx < hidden) return set_error(B200Q_ERR_INVALID, "bad shape");
     const int pairs = (int)pad_to(ffn, 8);
-    if ((long long)experts * 2 * pairs > INT_MAX || (long long)experts * hidden > INT_MAX) return set_error(B200Q_ERR_UNSUPPORTED, "matrices of 2^31 rows in all");
+    if ((long long)experts * 2 * pairs > INT_MAX - 512 || (long long)experts * hidden > INT_MAX - 512) return set_error(B200Q_ERR_UNSUPPORTED, "matrices of 2^31 rows in all");
     if (tokens == 0) return B200Q_OK;
     if (!x || !ids || !weights || !gate_up || !gate_up_scales || !down || !down_scales || !out || !workspace) return set_error(B200Q_ERR_INVALID, "null pointer");
     if (!aligned(workspace, 128)) return set_error(B200Q_ERR_INVALID, "the workspace must be 128-byte aligned");
@@ -194,15 +197,14 @@ int b200q_int8_experts(int elem, int activation, const void* x, long long ldx, c
     const ExpertsWorkspace w = experts_workspace(workspace, elem, slots, experts, hidden, ffn);
     if (workspace_bytes < w.bytes) return set_error(B200Q_ERR_TOO_LARGE, "workspace too small");
     cudaStream_t s = (cudaStream_t)stream;
-    cudaError_t e = route_sort(ids, id_bytes == 8, slots, experts, w.order, w.offsets, w.position, s);
-    if (e == cudaSuccess) e = int8_quantize_rows(elem, x, ldx, w.xq, w.ldx, w.xs, tokens, hidden, w.position, topk, nullptr, s, true);
     const Int8Product up{w.xq, w.xs, static_cast<const int8_t*>(gate_up), gate_up_scales, w.hidden, w.offsets, slots, 2 * pairs, hidden, (int)w.ldx, (int)w.ldx, experts, activation, ffn, w.ldh, status_ptr()};
-    if (e == cudaSuccess) e = int8_product(elem, up, s, true);
-    if (e == cudaSuccess) e = int8_quantize_rows(elem, w.hidden, w.ldh, w.hq, w.ldh, w.hs, slots, ffn, nullptr, 1, w.offsets + experts, s, true);
     const Int8Product dn{w.hq, w.hs, static_cast<const int8_t*>(down), down_scales, w.y, w.offsets, slots, hidden, ffn, (int)w.ldh, (int)w.ldh, experts, INT8_ACT_NONE, hidden, w.ldy, status_ptr()};
-    if (e == cudaSuccess) e = int8_product(ELEM_F32, dn, s, true);
-    if (e == cudaSuccess) e = route_combine(ELEM_F32, elem, w.y, w.ldy, w.position, weights, out, tokens, topk, hidden, s, true);
-    return cuda_result(e);
+    if (const int rc = cuda_result(route_sort(ids, id_bytes == 8, slots, experts, w.order, w.offsets, w.position, s))) return rc;
+    if (const int rc = cuda_result(int8_quantize_rows(elem, x, ldx, w.xq, w.ldx, w.xs, tokens, hidden, w.position, topk, nullptr, s, true))) return rc;
+    if (const int rc = int8_product(elem, up, s, true)) return rc;
+    if (const int rc = cuda_result(int8_quantize_rows(elem, w.hidden, w.ldh, w.hq, w.ldh, w.hs, slots, ffn, nullptr, 1, w.offsets + experts, s, true))) return rc;
+    if (const int rc = int8_product(ELEM_F32, dn, s, true)) return rc;
+    return cuda_result(route_combine(ELEM_F32, elem, w.y, w.ldy, w.position, weights, out, tokens, topk, hidden, s, true));
 }
 
 }  // extern "C"

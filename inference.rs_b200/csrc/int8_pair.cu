@@ -1,0 +1,356 @@
+// Products of int8 rows on the tensor cores: tcgen05.mma.cta_group::2, kind::i8. A pair of SMs owns a tile of 256 weight rows x up to 256
+// tokens; each SM holds 128 of the weight rows and half of the tokens in shared memory, brought there by TMA in 128-byte pieces of k,
+// and the sums stay in tensor memory as 32-bit integers until the epilogue scales them by token and channel.
+//
+// The weights sit on the M side of the instruction: its N side, the tokens, goes in steps of 32, so a ragged number of tokens wastes
+// little. With several matrices (experts) the tiles of all of them form one list, and a tile holds rows of one expert; where an expert's
+// rows begin and end is read on the device. A tile's boxes may reach into the next expert's rows: those columns are computed and not
+// stored. Two accumulators: the epilogue of one tile runs beside the product of the next.
+//
+// Every wait is bounded; a wait that gives up records a code in the device status word, work is skipped, and the kernel still frees its
+// TMEM columns before it returns.
+#include <cuda.h>
+
+#include "int8.cuh"
+#include "tcgen05.cuh"
+
+namespace b200q {
+
+constexpr int I8P_ROWS = 128;      // weight rows of one CTA = TMEM lanes
+constexpr int I8P_TOKENS = 256;    // tokens of a tile at most = TMEM columns of one accumulator
+constexpr int I8P_BK = 128;        // k per stage: one 128-byte swizzled row
+constexpr int I8P_MAX_STAGES = 12;
+constexpr int I8P_A_BYTES = I8P_ROWS * I8P_BK;
+constexpr int I8P_THREADS = 256;   // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warps 4-7 epilogue
+constexpr int I8P_TMEM_COLS = 512;
+
+struct Int8PairParams {
+    Int8Product p;
+    int bn;       // tokens per tile at most: a multiple of 32
+    int stages;
+    int tiles_n;  // weight tiles of 256 rows, of one matrix
+};
+struct Int8PairBarriers {
+    uint64_t full[I8P_MAX_STAGES], empty[I8P_MAX_STAGES];
+    uint64_t tmem_full[2], tmem_empty[2];
+    uint32_t tmem_base;
+    int scan[I8P_THREADS / 32];
+};
+static size_t i8p_smem(int stages, int bn, int experts) {
+    return 1024 + (size_t)stages * (I8P_A_BYTES + bn / 2 * I8P_BK) + sizeof(Int8PairBarriers) + (experts > 1 ? 8 * (size_t)(experts + 1) : 0);
+}
+
+// Where a tile lies: its weight tile, its expert, its tokens.
+struct Int8Tile {
+    int tn, e, row0, toks;
+};
+struct Int8TileList {
+    const int* start;    // shared memory: tiles before each expert's, experts + 1 of them (null: one matrix)
+    const int* offsets;  // shared memory
+    int experts, rows, bn, tiles_n, ntiles, at;
+    // called by whole warps, with tiles that do not fall
+    __device__ __forceinline__ Int8Tile find(int tile, int lane) {
+        Int8Tile t;
+        int first = 0, count = rows;
+        t.e = 0;
+        if (start != nullptr) {
+            for (;; at += 32) {
+                const int i = at + lane + 1;
+                const unsigned above = __ballot_sync(0xffffffffu, i > experts || start[i] > tile);
+                if (above != 0) {
+                    t.e = at + __ffs(above) - 1;
+                    break;
+                }
+            }
+            tile -= start[t.e];
+            first = offsets[t.e];
+            count = offsets[t.e + 1] - first;
+        }
+        const int tiles_m = (count + bn - 1) / bn;
+        t.tn = tile / tiles_m;
+        const int tm = tile - t.tn * tiles_m;
+        t.row0 = first + tm * bn;
+        t.toks = min(bn, count - tm * bn);
+        return t;
+    }
+};
+__device__ __forceinline__ int tile_columns(int toks) { return (toks + 31) & ~31; }  // N of the instruction
+
+template <typename OutT, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
+    int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Int8PairParams pp) {
+    extern __shared__ uint8_t i8p_smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(i8p_smem_raw) + 1023) & ~(uintptr_t)1023);
+    const Int8Product& p = pp.p;
+    uint8_t* a_stages = smem;
+    const int stages = pp.stages, half = pp.bn / 2, b_bytes = half * I8P_BK;  // bytes: a multiple of 1024
+    uint8_t* b_stages = smem + stages * I8P_A_BYTES;
+    Int8PairBarriers* bars = reinterpret_cast<Int8PairBarriers*>(b_stages + stages * b_bytes);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int nkb = (p.k + I8P_BK - 1) / I8P_BK;
+    const uint32_t stage_bytes = 2u * (I8P_A_BYTES + (uint32_t)b_bytes);  // both CTAs' operands of a stage
+
+    if (tid == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(&bars->full[s], 1);
+            mbar_init(&bars->empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&bars->tmem_full[s], 1);
+            mbar_init(&bars->tmem_empty[s], 8);  // four epilogue warps of each CTA
+        }
+        mbar_init_fence();
+    }
+    if (warp == 2) tmem_alloc_pair(&bars->tmem_base, I8P_TMEM_COLS);
+    grid_dependency_wait();  // the rows, and where the experts' begin, are the work of the launch before
+    grid_launch_dependents();
+
+    Int8TileList list{nullptr, nullptr, p.experts, p.rows, pp.bn, pp.tiles_n, 0, 0};
+    if (p.experts > 1) {
+        int* offsets = reinterpret_cast<int*>(bars + 1);
+        int* start = offsets + p.experts + 1;
+        for (int i = tid; i <= p.experts; i += I8P_THREADS) offsets[i] = min(max(p.offsets[i], 0), p.rows);
+        __syncthreads();
+        const int per = (p.experts + I8P_THREADS - 1) / I8P_THREADS, e0 = tid * per, e1 = min(e0 + per, p.experts);
+        int sum = 0;
+        for (int e = e0; e < e1; ++e) sum += (max(offsets[e + 1] - offsets[e], 0) + pp.bn - 1) / pp.bn * pp.tiles_n;
+        int upto = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += v;
+        }
+        if (lane == 31) bars->scan[warp] = upto;
+        __syncthreads();
+        int before = upto - sum;
+        for (int w = 0; w < warp; ++w) before += bars->scan[w];
+        for (int e = e0; e < e1; ++e) {
+            start[e] = before;
+            before += (max(offsets[e + 1] - offsets[e], 0) + pp.bn - 1) / pp.bn * pp.tiles_n;
+            if (e == p.experts - 1) start[p.experts] = before;
+        }
+        __syncthreads();
+        list.start = start;
+        list.offsets = offsets;
+        list.ntiles = start[p.experts];
+    } else {
+        if (p.offsets != nullptr) list.rows = min(max(p.offsets[1], 0), p.rows);
+        list.ntiles = (list.rows + pp.bn - 1) / pp.bn * pp.tiles_n;
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // the other CTA's barriers exist before anything arrives at them
+    tc_fence_after();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+    const int ntiles = list.ntiles;
+
+    if (warp == 0) {
+        // ---------------- TMA: this CTA's 128 weight rows and half of the tokens; the leader's barrier counts both CTAs' bytes ----
+        int s = 0, g = 0;
+        uint32_t ph = 1;
+        bool ok = true;
+        const uint32_t full0 = map_to_rank(&bars->full[0], 0);
+        for (int tile = pair; tile < ntiles && ok; tile += npairs) {
+            const Int8Tile t = list.find(tile, lane);
+            const int row = t.e * p.n + t.tn * 2 * I8P_ROWS + (int)rank * I8P_ROWS, token = t.row0 + (int)rank * (tile_columns(t.toks) / 2);
+            for (int kb = 0; kb < nkb; ++kb, ++g) {
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars->empty[s], ph));
+                if (!ok) {
+                    if (lane == 0) record_failure(p.status, STATUS_WAIT_EMPTY_TIMEOUT, g);
+                    break;
+                }
+                if (elect_one()) {
+                    if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], stage_bytes);
+                    tma_load_2d_pair(a_stages + (size_t)s * I8P_A_BYTES, &tmap_w, kb * I8P_BK, row, full0 + 8u * s);
+                    tma_load_2d_pair(b_stages + (size_t)s * b_bytes, &tmap_x, kb * I8P_BK, token, full0 + 8u * s);
+                }
+                __syncwarp();
+                if (++s == stages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+        // the leader waits for its last copies before the CTAs may exit (they are counted on its barriers; the MMAs have
+        // consumed them unless something gave up)
+        if (!ok && rank == 0) {
+            for (int q = 0; q < min(g, stages); ++q) {
+                if (s == 0) { s = stages - 1; ph ^= 1u; } else --s;
+                if (!mbar_wait_bounded(&bars->full[s], ph ^ 1u)) {
+                    if (lane == 0) record_failure(p.status, STATUS_WAIT_DRAIN_TIMEOUT, q);
+                    break;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer: an elected lane of the leader, for both SMs ----------------
+        if (rank == 0) {
+            const uint64_t da0 = make_smem_desc_sw128(smem_u32(a_stages)), db0 = make_smem_desc_sw128(smem_u32(b_stages));
+            int s = 0, ti = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int tile = pair; tile < ntiles && ok; tile += npairs, ++ti) {
+                const int buf = ti & 1;
+                const uint32_t idesc = make_idesc_i8(2 * I8P_ROWS, tile_columns(list.find(tile, lane).toks));
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars->tmem_empty[buf], ((ti >> 1) & 1) ^ 1));
+                if (!ok) {
+                    if (lane == 0) record_failure(p.status, STATUS_WAIT_MMA_TIMEOUT, 2000 + ti);
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem_base + buf * I8P_TOKENS;
+                for (int kb = 0; kb < nkb; ++kb) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars->full[s], ph));
+                    if (!ok) {
+                        if (lane == 0) record_failure(p.status, STATUS_WAIT_FULL_TIMEOUT, kb);
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint64_t da = da0 + (uint64_t)(s * (I8P_A_BYTES >> 4)), db = db0 + (uint64_t)(s * (b_bytes >> 4));
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < I8P_BK / 32; ++k) tc_mma_i8_pair(d, da + 2 * k, db + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                        tc_commit_pair(&bars->empty[s]);  // frees the stage in both CTAs when these MMAs have read it
+                        if (kb == nkb - 1) tc_commit_pair(&bars->tmem_full[buf]);
+                    }
+                    __syncwarp();
+                    if (++s == stages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+        }
+    } else if (warp >= 4) {
+        // ---------------- epilogue: thread = weight row, 32 tokens at a time; a warp's store is 32 neighbouring outputs ----------------
+        const int quarter = warp & 3;
+        bool ok = true;
+        int ti = 0;
+        for (int tile = pair; tile < ntiles; tile += npairs, ++ti) {
+            const int buf = ti & 1;
+            const Int8Tile t = list.find(tile, lane);
+            const int n = t.tn * 2 * I8P_ROWS + (int)rank * I8P_ROWS + quarter * 32 + lane;
+            const float ws = n < p.n ? p.ws[(long long)t.e * p.n + n] : 0.0f;
+            if (!mbar_wait_bounded(&bars->tmem_full[buf], (ti >> 1) & 1)) {
+                record_failure(p.status, STATUS_WAIT_MMA_TIMEOUT, ti);
+                ok = false;
+            }
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * I8P_TOKENS;
+            OutT* y = static_cast<OutT*>(p.y) + (long long)t.row0 * p.ldy;
+            for (int c = 0; c < t.toks; c += 32) {
+                const float xs = c + lane < t.toks ? p.xs[t.row0 + c + lane] : 0.0f;
+                uint32_t acc[32];
+                tmem_ld_32x32(taddr + c, acc);
+                float v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = (float)(int)acc[j] * __shfl_sync(0xffffffffu, xs, j) * ws;
+                if constexpr (!GATED) {
+                    if (n < p.n) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (c + j < t.toks) y[(long long)(c + j) * p.ldy + n] = from_float<OutT>(v[j]);
+                    }
+                } else {
+                    // rows 8.. of 16 hold up, the others gate: the lane of a gate row takes tokens 0..15, that of its up row 16..31
+                    const bool is_up = (lane & 8) != 0;
+                    const int col = (n >> 4) * 8 + (n & 7);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const float other = __shfl_xor_sync(0xffffffffu, is_up ? v[j] : v[16 + j], 8);
+                        const float gate = is_up ? other : v[j], up = is_up ? v[16 + j] : other;
+                        const int tok = c + (is_up ? 16 + j : j);
+                        if (col < p.n_out && tok < t.toks) y[(long long)tok * p.ldy + col] = from_float<OutT>(int8_activate(gate, p.act) * up);
+                    }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(&bars->tmem_empty[buf], 0));  // the accumulator may be reused
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // neither CTA leaves while the other may still read its operands or arrive at its barriers
+    if (warp == 2) tmem_dealloc_pair(tmem_base, I8P_TMEM_COLS);
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------------------
+// Tokens per tile. One matrix: the height with the least waves x height, as tiles go out in waves of one per CTA pair; a wave takes as
+// long as its tile is high, but no less than a tile of about 148 tokens, and some 24 tokens' worth to fill and drain. Several: a bit
+// more than an expert has on average.
+static int int8_token_tile(const Int8Product& p, int tiles_n) {
+    if (p.experts > 1) {
+        const int per = p.rows / p.experts, bn = (per + per / 4 + 16 + 31) & ~31;
+        return bn < I8P_TOKENS ? bn : I8P_TOKENS;
+    }
+    const int pairs = runtime_info().sm_count / 2;
+    long long best = 0;
+    int best_bn = 0;
+    for (int tm = (p.rows + I8P_TOKENS - 1) / I8P_TOKENS, last = 0;; ++tm) {
+        const int bn = (((p.rows + tm - 1) / tm) + 31) & ~31;
+        if (best_bn != 0 && bn < 128) break;
+        if (bn == last) continue;
+        last = bn;
+        const long long waves = ((long long)((p.rows + bn - 1) / bn) * tiles_n + pairs - 1) / pairs;
+        const long long cost = waves * ((bn > 148 ? bn : 148) + 24);
+        if (best_bn == 0 || cost * 100 < best * 95) {
+            best = cost;
+            best_bn = bn;
+        }
+    }
+    return best_bn;
+}
+
+template <typename OutT, bool GATED> static int pair_t(const Int8Product& p, cudaStream_t s, bool dependent) {
+    Int8PairParams pp{};
+    pp.p = p;
+    pp.tiles_n = (p.n + 2 * I8P_ROWS - 1) / (2 * I8P_ROWS);
+    pp.bn = int8_token_tile(p, pp.tiles_n);
+    pp.stages = I8P_MAX_STAGES;
+    while (i8p_smem(pp.stages, pp.bn, p.experts) > (size_t)runtime_info().smem_optin - 1024) --pp.stages;
+    const cuuint64_t kp = (cuuint64_t)((p.k + 15) & ~15);
+    CUtensorMap map_w, map_x;
+    {
+        const cuuint64_t dims[2] = {kp, (cuuint64_t)p.experts * p.n};
+        const cuuint32_t box[2] = {I8P_BK, I8P_ROWS};
+        if (encode_tiled_2d_cached(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.wq, dims, (cuuint64_t)p.ldw, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != CUDA_SUCCESS)
+            return set_error(B200Q_ERR_INVALID, "no tensor map for the weights");
+    }
+    {
+        const cuuint64_t dims[2] = {kp, (cuuint64_t)p.rows};
+        const cuuint32_t box[2] = {I8P_BK, (cuuint32_t)(pp.bn / 2)};
+        if (encode_tiled_2d_cached(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.xq, dims, (cuuint64_t)p.ldx, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != CUDA_SUCCESS)
+            return set_error(B200Q_ERR_INVALID, "no tensor map for the activations");
+    }
+    constexpr auto kernel = int8_pair_kernel<OutT, GATED>;
+    cudaError_t e = allow_full_smem<kernel>();
+    if (e == cudaSuccess) {
+        const int pairs = runtime_info().sm_count / 2;
+        // at most one tile more per expert than the rows fill
+        const long long tiles = ((long long)p.rows / pp.bn + p.experts) * pp.tiles_n;
+        const unsigned grid = 2u * (unsigned)(tiles < pairs ? tiles : pairs);
+        e = launch_kernel(kernel, dim3(grid, 1, 1), I8P_THREADS, i8p_smem(pp.stages, pp.bn, p.experts), s, dependent, map_w, map_x, pp);
+    }
+    return e == cudaSuccess ? B200Q_OK : set_error((int)e, cudaGetErrorString(e));
+}
+template <typename OutT> static int pair_out(const Int8Product& p, cudaStream_t s, bool dependent) {
+    return p.act == INT8_ACT_NONE ? pair_t<OutT, false>(p, s, dependent) : pair_t<OutT, true>(p, s, dependent);
+}
+
+bool int8_pair_pays(const Int8Product& p) { return encode_tiled_fn() != nullptr && p.rows > 64 * p.experts; }
+
+int int8_product_pair(int elem, const Int8Product& p, cudaStream_t s, bool dependent) {
+    if (elem == ELEM_F32) return pair_out<float>(p, s, dependent);
+    if (elem == ELEM_F16) return pair_out<__half>(p, s, dependent);
+    return pair_out<__nv_bfloat16>(p, s, dependent);
+}
+
+}  // namespace b200q
