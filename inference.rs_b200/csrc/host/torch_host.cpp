@@ -10,8 +10,11 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/_to_copy.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>  // C++ exceptions become the Python ones torch raises itself (OutOfMemoryError among them)
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdint>
@@ -45,6 +48,19 @@ using GluFn = void (*)(const void*, const void*, const void*, void*, int, int, i
 using QuantMmqFn = void (*)(const void*, const int32_t*, void*, int, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, void*);
 using MmqFn = void (*)(void*, const void*, const void*, void*, int64_t, int64_t, int64_t, int64_t, int64_t, int, int, int64_t, int, int, void*);
 
+using Int8QuantizeFn = int (*)(int, const void*, int64_t, void*, int64_t, float*, int64_t, int, void*);
+using Int8DequantizeFn = int (*)(int, const void*, int64_t, const float*, void*, int64_t, int, void*);
+using Int8BytesFn = int64_t (*)(int, int);
+using Int8MatmulFn = int (*)(int, const void*, const void*, const float*, void*, int, int, int, int64_t, int64_t, int64_t, void*, int64_t, void*);
+using Int8ExpertsBytesFn = int64_t (*)(int, int, int, int, int, int);
+using Int8ExpertsFn = int (*)(int, int, const void*, int64_t, const void*, int, const float*, const void*, const float*, const void*, const float*, void*, int, int, int,
+                              int, int, void*, int64_t, void*);
+using RouteSortFn = int (*)(const void*, int, int, int, int*, int*, int*, void*);
+using RouteDispatchFn = int (*)(int, const void*, int64_t, const int*, const int*, int, void*, int, int, int, void*);
+using RouteCombineFn = int (*)(int, int, const void*, int64_t, const int*, const float*, void*, int, int, int, void*);
+using RouteCombineGradFn = int (*)(int, int, const void*, int64_t, const void*, int64_t, const int*, const int*, int, const float*, void*, float*, int, int, int, void*);
+using LastErrorFn = const char* (*)();
+
 // indexed by type (0 q8_0, 1 q4_k, 2 q6_k) and element type
 struct Abi {
     GemvFn gemv;
@@ -63,6 +79,17 @@ struct Abi {
     GluFn glu[3][3];
     QuantMmqFn quant_mmq[2];  // D4, DS4
     MmqFn mmq[3];
+    Int8QuantizeFn int8_quantize;
+    Int8DequantizeFn int8_dequantize;
+    Int8BytesFn int8_matmul_bytes;
+    Int8MatmulFn int8_matmul;
+    Int8ExpertsBytesFn int8_experts_bytes;
+    Int8ExpertsFn int8_experts;
+    RouteSortFn route_sort;
+    RouteDispatchFn route_dispatch;
+    RouteCombineFn route_combine;
+    RouteCombineGradFn route_combine_grad;
+    LastErrorFn last_error;
 } abi{};
 PyObject* check_fn = nullptr;          // kernel_library.check(rc, what): raises for a non-zero status
 PyObject* launch_failed_fn = nullptr;  // raises for a status kept by a void launcher
@@ -99,6 +126,17 @@ const AbiEntry abi_entries[] = {
 #undef B200Q_HOST_TYPE
     {"launch_mmq_quantize_q8_1_D4", (void**)&abi.quant_mmq[0]},
     {"launch_mmq_quantize_q8_1_DS4", (void**)&abi.quant_mmq[1]},
+    {"b200q_int8_quantize", (void**)&abi.int8_quantize},
+    {"b200q_int8_dequantize", (void**)&abi.int8_dequantize},
+    {"b200q_int8_matmul_workspace_bytes", (void**)&abi.int8_matmul_bytes},
+    {"b200q_int8_matmul", (void**)&abi.int8_matmul},
+    {"b200q_int8_experts_workspace_bytes", (void**)&abi.int8_experts_bytes},
+    {"b200q_int8_experts", (void**)&abi.int8_experts},
+    {"b200q_route_sort", (void**)&abi.route_sort},
+    {"b200q_route_dispatch", (void**)&abi.route_dispatch},
+    {"b200q_route_combine", (void**)&abi.route_combine},
+    {"b200q_route_combine_grad", (void**)&abi.route_combine_grad},
+    {"b200q_last_error", (void**)&abi.last_error},
 };
 
 int type_index(long type) { return type == TYPE_Q8_0 ? 0 : (type == TYPE_Q4_K ? 1 : (type == TYPE_Q6_K ? 2 : -1)); }
@@ -133,6 +171,16 @@ bool int_args(PyObject* const* args, std::initializer_list<std::pair<int, long*>
 }
 Tensor empty(at::IntArrayRef size, ScalarType t, const Tensor& like) { return at::detail::empty_cuda(size, t, like.device(), std::nullopt); }
 PyObject* none() { Py_RETURN_NONE; }
+// a tuple that takes its items over
+PyObject* tuple_of(std::initializer_list<PyObject*> items) {
+    PyObject* tuple = PyTuple_New((Py_ssize_t)items.size());
+    Py_ssize_t i = 0;
+    for (PyObject* o : items) {
+        if (tuple != nullptr) PyTuple_SET_ITEM(tuple, i++, o);
+        else Py_XDECREF(o);
+    }
+    return tuple;
+}
 // launches may block (a full queue, a first load of a kernel): other Python threads go on meanwhile
 struct NoGil {
     PyThreadState* state = PyEval_SaveThread();
@@ -453,6 +501,253 @@ PyObject* py_get_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- int8 rows, experts, routing ----
+// These launch on the current stream of their tensors' device.
+constexpr int64_t INT8_ROW_ALIGN = 16, MOST = 2147483647 - 65536;
+
+struct OnDevice {
+    c10::cuda::CUDAGuard guard;
+    void* stream;
+    explicit OnDevice(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+};
+bool same_device(const Tensor& a, std::initializer_list<const Tensor*> others) {
+    for (const Tensor* t : others)
+        if (t->device() != a.device()) return false;
+    return true;
+}
+bool of(const Tensor* t, ScalarType type) { return cuda_contiguous(t) && t->scalar_type() == type; }
+// rows of unit stride that do not overlap
+bool row_stride(const Tensor& t, int64_t& ld) {
+    if (t.dim() != 2) return false;
+    if (t.is_contiguous()) {
+        ld = t.size(1);
+        return true;
+    }
+    ld = t.stride(0);
+    return t.size(0) > 1 && t.size(1) > 1 && t.stride(1) == 1 && ld >= t.size(1);
+}
+bool wants_grad(const Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+// in a backward pass there is no interpreter to raise with
+void require(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with status ", rc, ": ", abi.last_error()); }
+
+// int8_forward(wq, scales, n, k, x): y = x . W^T
+PyObject* py_int8_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    long n, k;
+    if (nargs != 5 || !int_args(args, {{2, &n}, {3, &k}})) return none();
+    const Tensor *w = tensor_arg(args[0]), *ws = tensor_arg(args[1]), *x = tensor_arg(args[4]);
+    if (!of(w, ScalarType::Char) || !of(ws, ScalarType::Float) || !cuda_contiguous(x) || x->dim() < 2 || x->size(-1) != k || k < 1 || n < 1 || n > MOST || wants_grad(*x)) return none();
+    const int64_t kp = pad(k, INT8_ROW_ALIGN), m = x->numel() / k;
+    const int elem = elem_of(x->scalar_type());
+    if (elem < 0 || m == 0 || m > MOST || w->dim() != 2 || w->size(0) != n || w->size(1) != kp || ws->numel() != n || !same_device(*x, {w, ws})) return none();
+    OnDevice on(*x);
+    c10::SmallVector<int64_t, 6> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = n;
+    Tensor y = empty(shape, x->scalar_type(), *x);
+    const int64_t bytes = abi.int8_matmul_bytes((int)m, (int)k);
+    const Tensor space = empty({bytes}, ScalarType::Byte, *x);
+    if (failed(call(abi.int8_matmul, elem, x->data_ptr(), w->data_ptr(), ws->data_ptr<float>(), y.data_ptr(), (int)m, (int)n, (int)k, (int64_t)k, kp, (int64_t)n, space.data_ptr(), bytes,
+                    on.stream),
+               "b200q_int8_matmul"))
+        return nullptr;
+    return THPVariable_Wrap(std::move(y));
+    END_HANDLE_TH_ERRORS
+}
+
+// int8_quantize(x): (q, scales) of a matrix's rows
+PyObject* py_int8_quantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    const Tensor* x = nargs == 1 ? tensor_arg(args[0]) : nullptr;
+    int64_t ld;
+    if (x == nullptr || !x->is_cuda() || !row_stride(*x, ld) || elem_of(x->scalar_type()) < 0 || x->numel() == 0 || x->size(0) > MOST || x->size(1) > MOST) return none();
+    OnDevice on(*x);
+    const int64_t m = x->size(0), k = x->size(1), kp = pad(k, INT8_ROW_ALIGN);
+    Tensor q = empty({m, kp}, ScalarType::Char, *x), scales = empty({m}, ScalarType::Float, *x);
+    if (failed(call(abi.int8_quantize, elem_of(x->scalar_type()), x->data_ptr(), ld, q.data_ptr(), kp, scales.data_ptr<float>(), m, (int)k, on.stream), "b200q_int8_quantize"))
+        return nullptr;
+    return tuple_of({THPVariable_Wrap(std::move(q)), THPVariable_Wrap(std::move(scales))});
+    END_HANDLE_TH_ERRORS
+}
+
+// int8_dequantize(q, scales, k, elem)
+PyObject* py_int8_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    long k, elem;
+    ScalarType t;
+    if (nargs != 4 || !int_args(args, {{2, &k}, {3, &elem}}) || !elem_scalar(elem, t)) return none();
+    const Tensor *q = tensor_arg(args[0]), *scales = tensor_arg(args[1]);
+    if (!of(q, ScalarType::Char) || !of(scales, ScalarType::Float) || q->dim() < 2 || k < 1 || q->size(-1) != pad(k, INT8_ROW_ALIGN) || q->numel() == 0 || !same_device(*q, {scales})) return none();
+    const int64_t rows = q->numel() / q->size(-1);
+    if (scales->numel() != rows || rows > MOST) return none();
+    OnDevice on(*q);
+    c10::SmallVector<int64_t, 6> shape(q->sizes().begin(), q->sizes().end());
+    shape.back() = k;
+    Tensor out = empty(shape, t, *q);
+    if (failed(call(abi.int8_dequantize, (int)elem, q->data_ptr(), q->size(-1), scales->data_ptr<float>(), out.data_ptr(), rows, (int)k, on.stream), "b200q_int8_dequantize")) return nullptr;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// int8_experts(x, ids, weights, gate_up, gate_up_scales, down, down_scales, ffn, activation)
+PyObject* py_int8_experts(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    long ffn, act;
+    if (nargs != 9 || !int_args(args, {{7, &ffn}, {8, &act}})) return none();
+    const Tensor* t[7];
+    for (int i = 0; i < 7; ++i)
+        if (!cuda_contiguous(t[i] = tensor_arg(args[i]))) return none();
+    const Tensor &x = *t[0], &ids = *t[1], &weights = *t[2], &gate_up = *t[3], &gus = *t[4], &down = *t[5], &ds = *t[6];
+    const int elem = elem_of(x.scalar_type());
+    if (elem < 0 || (ids.scalar_type() != ScalarType::Int && ids.scalar_type() != ScalarType::Long) || weights.scalar_type() != ScalarType::Float ||
+        gate_up.scalar_type() != ScalarType::Char || down.scalar_type() != ScalarType::Char || gus.scalar_type() != ScalarType::Float || ds.scalar_type() != ScalarType::Float ||
+        x.dim() < 2 || ids.dim() != x.dim() || ids.sizes() != weights.sizes() || gate_up.dim() != 3 || down.dim() != 3 || ffn < 1 || x.numel() == 0 || ids.numel() == 0 ||
+        wants_grad(x) || wants_grad(weights) || !same_device(x, {t[1], t[2], t[3], t[4], t[5], t[6]}))
+        return none();
+    for (int64_t i = 0; i + 1 < x.dim(); ++i)
+        if (x.size(i) != ids.size(i)) return none();
+    const int64_t hidden = x.size(-1), tokens = x.numel() / hidden, topk = ids.size(-1), experts = gate_up.size(0), p = pad(ffn, 8);
+    if (tokens * topk > MOST || gate_up.size(1) != 2 * p || gate_up.size(2) != pad(hidden, INT8_ROW_ALIGN) || down.size(0) != experts || down.size(1) != hidden ||
+        down.size(2) != pad(ffn, INT8_ROW_ALIGN) || gus.numel() != experts * 2 * p || ds.numel() != experts * hidden)
+        return none();
+    OnDevice on(x);
+    Tensor out = empty(x.sizes(), x.scalar_type(), x);
+    const int64_t bytes = abi.int8_experts_bytes(elem, (int)tokens, (int)topk, (int)experts, (int)hidden, (int)ffn);
+    const Tensor space = empty({bytes}, ScalarType::Byte, x);
+    if (failed(call(abi.int8_experts, elem, (int)act, x.data_ptr(), hidden, ids.data_ptr(), (int)ids.element_size(), weights.data_ptr<float>(), gate_up.data_ptr(), gus.data_ptr<float>(),
+                    down.data_ptr(), ds.data_ptr<float>(), out.data_ptr(), (int)tokens, (int)experts, (int)topk, (int)hidden, (int)ffn, space.data_ptr(), bytes, on.stream),
+               "b200q_int8_experts"))
+        return nullptr;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// route_sort(ids, experts): (order, offsets, position)
+PyObject* py_route_sort(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    long experts;
+    if (nargs != 2 || !int_arg(args[1], experts) || experts < 1 || experts > 1024) return none();
+    const Tensor* ids = tensor_arg(args[0]);
+    if (!cuda_contiguous(ids) || (ids->scalar_type() != ScalarType::Int && ids->scalar_type() != ScalarType::Long) || ids->numel() > MOST) return none();
+    OnDevice on(*ids);
+    const int64_t slots = ids->numel();
+    Tensor order = empty({slots}, ScalarType::Int, *ids), offsets = empty({experts + 1}, ScalarType::Int, *ids), position = empty(ids->sizes(), ScalarType::Int, *ids);
+    if (failed(call(abi.route_sort, ids->data_ptr(), (int)ids->element_size(), (int)slots, (int)experts, order.data_ptr<int>(), offsets.data_ptr<int>(), position.data_ptr<int>(), on.stream),
+               "b200q_route_sort"))
+        return nullptr;
+    return tuple_of({THPVariable_Wrap(std::move(order)), THPVariable_Wrap(std::move(offsets)), THPVariable_Wrap(std::move(position))});
+    END_HANDLE_TH_ERRORS
+}
+
+Tensor combine(const Tensor& rows, int64_t ld, const Tensor& position, const float* weights, ScalarType type) {
+    const int64_t topk = position.size(-1), tokens = position.numel() / topk;
+    OnDevice on(rows);
+    Tensor out = empty({tokens, rows.size(1)}, type, rows);
+    require(abi.route_combine(elem_of(rows.scalar_type()), elem_of(type), rows.data_ptr(), ld, position.data_ptr<int>(), weights, out.data_ptr(), (int)tokens, (int)topk, (int)rows.size(1),
+                              on.stream),
+            "b200q_route_combine");
+    return out;
+}
+Tensor dispatch(const Tensor& x, int64_t ld, const Tensor& position, const Tensor& offsets) {
+    const int64_t topk = position.size(-1);
+    OnDevice on(x);
+    Tensor rows = empty({x.size(0) * topk, x.size(1)}, x.scalar_type(), x);
+    require(abi.route_dispatch(elem_of(x.scalar_type()), x.data_ptr(), ld, position.data_ptr<int>(), offsets.data_ptr<int>(), (int)offsets.numel() - 1, rows.data_ptr(), (int)x.size(0),
+                               (int)topk, (int)x.size(1), on.stream),
+            "b200q_route_dispatch");
+    return rows;
+}
+// a gradient as the kernels take it
+Tensor grad_rows_of(const Tensor& g, int64_t& ld) {
+    if (row_stride(g, ld)) return g;
+    Tensor c = g.contiguous();
+    ld = c.size(1);
+    return c;
+}
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& position, const Tensor& offsets) {
+        ctx->save_for_backward({position});
+        ctx->saved_data["type"] = (int64_t)x.scalar_type();
+        int64_t ld;
+        TORCH_CHECK(row_stride(x, ld));  // the caller has looked
+        return dispatch(x, ld, position, offsets);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const Tensor position = ctx->get_saved_variables()[0];
+        TORCH_CHECK(!c10::GradMode::is_enabled(), "the gradient of dispatch cannot be differentiated again (create_graph)");
+        int64_t ld;
+        const Tensor g = grad_rows_of(grads[0], ld);
+        return {combine(g, ld, position, nullptr, (ScalarType)ctx->saved_data["type"].toInt()), Tensor(), Tensor()};
+    }
+};
+struct CombineFunction : torch::autograd::Function<CombineFunction> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& rows, const Tensor& weights, const Tensor& position, const Tensor& offsets, int64_t type) {
+        ctx->save_for_backward({rows, weights, position, offsets});
+        int64_t ld;
+        TORCH_CHECK(row_stride(rows, ld));
+        return combine(rows, ld, position, weights.data_ptr<float>(), (ScalarType)type);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &rows = saved[0], &weights = saved[1], &position = saved[2], &offsets = saved[3];
+        TORCH_CHECK(!c10::GradMode::is_enabled(), "the gradient of combine cannot be differentiated again (create_graph)");
+        int64_t ldg, ldr;
+        const Tensor g = grad_rows_of(grads[0], ldg);
+        TORCH_CHECK(row_stride(rows, ldr));
+        const int64_t topk = position.size(-1), tokens = position.numel() / topk;
+        OnDevice on(g);
+        Tensor grad_rows, grad_weights;
+        if (ctx->needs_input_grad(0)) grad_rows = empty({rows.size(0), rows.size(1)}, rows.scalar_type(), rows);
+        if (ctx->needs_input_grad(1)) grad_weights = empty(weights.sizes(), ScalarType::Float, rows);
+        require(abi.route_combine_grad(elem_of(g.scalar_type()), elem_of(rows.scalar_type()), g.data_ptr(), ldg, rows.data_ptr(), ldr, position.data_ptr<int>(), offsets.data_ptr<int>(),
+                                       (int)offsets.numel() - 1, weights.data_ptr<float>(), grad_rows.defined() ? grad_rows.data_ptr() : nullptr,
+                                       grad_weights.defined() ? grad_weights.data_ptr<float>() : nullptr, (int)tokens, (int)topk, (int)rows.size(1), on.stream),
+                "b200q_route_combine_grad");
+        return {grad_rows, grad_weights, Tensor(), Tensor(), Tensor()};
+    }
+};
+
+// route_dispatch(x, position, offsets), differentiable
+PyObject* py_route_dispatch(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (nargs != 3) return none();
+    const Tensor *x = tensor_arg(args[0]), *position = tensor_arg(args[1]), *offsets = tensor_arg(args[2]);
+    int64_t ld;
+    if (x == nullptr || !x->is_cuda() || !row_stride(*x, ld) || elem_of(x->scalar_type()) < 0 || x->numel() == 0 || x->size(1) > MOST || !of(position, ScalarType::Int) || position->dim() < 2 ||
+        position->numel() == 0 || position->numel() / position->size(-1) != x->size(0) || !of(offsets, ScalarType::Int) || offsets->numel() < 2 || !same_device(*x, {position, offsets}))
+        return none();
+    Tensor rows;
+    {
+        NoGil nogil;
+        rows = wants_grad(*x) ? DispatchFunction::apply(*x, *position, *offsets) : dispatch(*x, ld, *position, *offsets);
+    }
+    return THPVariable_Wrap(std::move(rows));
+    END_HANDLE_TH_ERRORS
+}
+
+// route_combine(rows, weights, position, offsets, elem), differentiable
+PyObject* py_route_combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    long elem;
+    ScalarType type;
+    if (nargs != 5 || !int_arg(args[4], elem) || !elem_scalar(elem, type)) return none();
+    const Tensor *rows = tensor_arg(args[0]), *weights = tensor_arg(args[1]), *position = tensor_arg(args[2]), *offsets = tensor_arg(args[3]);
+    int64_t ld;
+    if (rows == nullptr || !rows->is_cuda() || !row_stride(*rows, ld) || elem_of(rows->scalar_type()) < 0 || rows->numel() == 0 || rows->size(1) > MOST || !of(weights, ScalarType::Float) ||
+        !of(position, ScalarType::Int) || position->dim() < 2 || position->sizes() != weights->sizes() || position->numel() != rows->size(0) || !of(offsets, ScalarType::Int) ||
+        offsets->numel() < 2 || !same_device(*rows, {weights, position, offsets}))
+        return none();
+    Tensor out;
+    {
+        NoGil nogil;
+        out = wants_grad(*rows) || wants_grad(*weights) ? CombineFunction::apply(*rows, *weights, *position, *offsets, (int64_t)type)
+                                                        : combine(*rows, ld, *position, weights->data_ptr<float>(), type);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 // bind(names, addresses, check, launch_failed)
 PyObject* py_bind(PyObject*, PyObject* args) {
     PyObject *addresses, *check, *launch_failed;
@@ -496,6 +791,13 @@ PyMethodDef methods[] = {
     B200Q_FAST("quantize", py_quantize),
     B200Q_FAST("dequantize", py_dequantize),
     B200Q_FAST("get_rows", py_get_rows),
+    B200Q_FAST("int8_forward", py_int8_forward),
+    B200Q_FAST("int8_quantize", py_int8_quantize),
+    B200Q_FAST("int8_dequantize", py_int8_dequantize),
+    B200Q_FAST("int8_experts", py_int8_experts),
+    B200Q_FAST("route_sort", py_route_sort),
+    B200Q_FAST("route_dispatch", py_route_dispatch),
+    B200Q_FAST("route_combine", py_route_combine),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "b200q_torch_host", "Native call path of the torch front end.", -1, methods, nullptr, nullptr, nullptr, nullptr};

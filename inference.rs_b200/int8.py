@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import torch
 
+from . import kernel_library as kl
 from . import ops
 from .dtypes import pad
 from .qmatmul import QTensor
@@ -63,6 +64,9 @@ class Int8Tensor:
 
     def dequantize(self, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values as a dense tensor of this shape."""
+        out = kl.host().int8_dequantize(self.data, self.scales, self.shape[-1], ops.elem_of(out_dtype))
+        if out is not None:
+            return out
         return ops.int8_dequantize(self.data.view(-1, self.data.shape[-1]), self.scales.view(-1), self.shape[-1], out_dtype).view(self.shape)
 
     @property
@@ -84,6 +88,15 @@ class Int8MatMul:
 
     def forward(self, xs: torch.Tensor) -> torch.Tensor:
         n, k = self.w.shape
+        y = kl.host().int8_forward(self.w.data, self.w.scales, n, k, xs)
+        if y is None:
+            y = self._forward(xs, n, k)
+        return y if self.b is None else y + self.b.to(y.dtype)
+
+    __call__ = forward
+
+    def _forward(self, xs: torch.Tensor, n: int, k: int) -> torch.Tensor:
+        """What the native path declines as it stands: errors among them."""
         if xs.dim() < 2:
             raise ValueError(f"input tensor has only one dimension {tuple(xs.shape)}")
         if not xs.is_contiguous():
@@ -93,10 +106,7 @@ class Int8MatMul:
         if xs.device != self.w.device:
             raise ValueError(f"input on {xs.device}, weights on {self.w.device}")
         _no_grad_through(xs)
-        y = ops.int8_matmul(xs.view(-1, k), self.w.data, self.w.scales).view(*xs.shape[:-1], n)
-        return y if self.b is None else y + self.b.to(y.dtype)
-
-    __call__ = forward
+        return ops.int8_matmul(xs.view(-1, k), self.w.data, self.w.scales).view(*xs.shape[:-1], n)
 
 
 class Int8Experts:
@@ -125,6 +135,10 @@ class Int8Experts:
     def forward(self, x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
         """x [..., hidden]; ids [..., slots] (int32 or int64) names each token's experts, weights [..., slots] their weights. A slot
         whose id is not one of 0..experts - 1 counts for nothing. -> [..., hidden] in x's type."""
+        out = kl.host().int8_experts(x, ids, weights, self.gate_up, self.gate_up_scales, self.down.data, self.down.scales, self.ffn,
+                                     ops.GLU_ACTIVATIONS[self.activation])
+        if out is not None:
+            return out
         if x.dim() < 2 or x.shape[-1] != self.hidden or ids.shape != weights.shape or tuple(ids.shape[:-1]) != tuple(x.shape[:-1]):
             raise ValueError(f"tokens {tuple(x.shape)}, ids {tuple(ids.shape)}, weights {tuple(weights.shape)} for a layer of width {self.hidden}")
         _no_grad_through(x, weights)

@@ -11,6 +11,7 @@ import math
 import torch
 from torch.autograd.function import once_differentiable
 
+from . import kernel_library as kl
 from . import ops
 
 
@@ -55,7 +56,8 @@ class TokenRouting:
         if ids.shape[-1] == 0:
             raise ValueError(f"tokens with no slots: {tuple(ids.shape)}")
         self.experts = int(experts)
-        self.order, self.offsets, self.position = ops.route_sort(ids, self.experts)
+        sorted_slots = kl.host().route_sort(ids, self.experts)
+        self.order, self.offsets, self.position = ops.route_sort(ids, self.experts) if sorted_slots is None else sorted_slots
 
     def _position2d(self) -> torch.Tensor:
         return self.position.view(math.prod(self.position.shape[:-1]), self.position.shape[-1])
@@ -64,6 +66,9 @@ class TokenRouting:
         """x [..., h], a row per token -> [slots, h], a row per slot in the order of the experts; rows behind the last expert's are zeros."""
         if tuple(x.shape[:-1]) != tuple(self.position.shape[:-1]):
             raise ValueError(f"tokens {tuple(x.shape)} for expert ids {tuple(self.position.shape)}")
+        rows = kl.host().route_dispatch(x, self.position, self.offsets) if x.dim() == 2 == self.position.dim() else None
+        if rows is not None:
+            return rows
         position = self._position2d()
         x2 = x.reshape(position.shape[0], x.shape[-1])
         if torch.is_grad_enabled() and x2.requires_grad:
@@ -76,8 +81,13 @@ class TokenRouting:
         expert's are not read."""
         if tuple(weights.shape) != tuple(self.position.shape):
             raise ValueError(f"weights {tuple(weights.shape)} for expert ids {tuple(self.position.shape)}")
-        position, out_dtype = self._position2d(), rows.dtype if out_dtype is None else out_dtype
-        w = weights.to(torch.float32).reshape(position.shape).contiguous()
+        out_dtype = rows.dtype if out_dtype is None else out_dtype
+        w = weights.to(torch.float32).contiguous()
+        out = kl.host().route_combine(rows, w, self.position, self.offsets, ops.elem_of(out_dtype))
+        if out is not None:
+            return out if weights.dim() == 2 else out.view(*weights.shape[:-1], rows.shape[-1])
+        position = self._position2d()
+        w = w.view(position.shape)
         if torch.is_grad_enabled() and (rows.requires_grad or w.requires_grad):
             out = _Combine.apply(rows, w, position, self.offsets, out_dtype)
         else:

@@ -10,6 +10,7 @@ import pytest
 import torch
 
 import inference_rs_b200 as pkg
+from inference_rs_b200 import kernel_library as kl
 from inference_rs_b200 import ops
 from gpu_util import assert_device_ok
 
@@ -17,6 +18,13 @@ pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 U = 2.0 ** -24
+
+
+@pytest.fixture(params=["native", "python"], autouse=True)
+def call_path(request, monkeypatch):
+    """Both call paths of the torch front end."""
+    if request.param == "python":
+        monkeypatch.setattr(kl, "_host", kl.NoNativePath())
 
 
 def rows64(x):

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 import inference_rs_b200 as pkg
+from inference_rs_b200 import kernel_library as kl
 from inference_rs_b200 import ops
 from gpu_util import assert_device_ok
 
@@ -16,6 +17,13 @@ pytestmark = pytest.mark.gpu
 
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 U = 2.0 ** -24
+
+
+@pytest.fixture(params=["native", "python"], autouse=True)
+def call_path(request, monkeypatch):
+    """Both call paths of the torch front end."""
+    if request.param == "python":
+        monkeypatch.setattr(kl, "_host", kl.NoNativePath())
 SHAPES = [(1, 1, 1, 1), (1, 8, 2, 64), (7, 128, 8, 100), (33, 60, 4, 1037), (300, 2, 1, 512), (513, 1024, 3, 24), (1000, 5, 6, 130), (64, 16, 16, 2048)]
 
 
@@ -157,6 +165,16 @@ def test_only_the_gradients_asked_for():
     assert torch.equal(torch.autograd.grad(r.combine(y.detach(), w).sum(), w)[0], both[1])
     with torch.no_grad():
         assert not r.combine(y, w).requires_grad and not r.dispatch(values(9, 8, torch.float32, 1).requires_grad_()).requires_grad
+
+
+def test_no_second_derivatives():
+    r = pkg.TokenRouting(choose(9, 4, 2, 0.0), 4)
+    y, w = values(18, 64, torch.float32, 1).requires_grad_(), torch.rand(9, 2, device="cuda").requires_grad_()
+    x = values(9, 64, torch.float32, 2).requires_grad_()
+    for out, inputs in ((r.combine(y, w), (y, w)), (r.dispatch(x), (x,))):
+        with pytest.raises(RuntimeError, match="differentiat"):
+            first = torch.autograd.grad((out ** 2).sum(), inputs, create_graph=True)
+            sum((g ** 2).sum() for g in first).backward()
 
 
 def test_in_graphs_and_on_other_streams():
