@@ -15,13 +15,20 @@ constexpr int INT8_MAX_EXPERTS = 1024;
 // Activation of a gated product, act(gate) * up, by the ids of the reference's host side
 // (crates/inference-quant/kernels/cuda/glu_activation.cuh:4-10); -1: the product is not gated.
 enum Int8Act : int { INT8_ACT_NONE = -1, INT8_ACT_SILU = 0, INT8_ACT_GELU = 1, INT8_ACT_RELU = 2, INT8_ACT_GELU_ERF = 3, INT8_ACT_SIGMOID = 4 };
+// Quotients by __fdividef: two units of the last place, and 0 where the divisor passes 2^126, which is where the value has vanished. An
+// IEEE division's way out of line kept the epilogue's values from overlapping: 54000 cycles for 256 x 256 of them where the product took
+// 16000.
 __device__ __forceinline__ float int8_activate(float x, int act) {
     switch (act) {
-        case INT8_ACT_GELU: return 0.5f * x * (1.0f + tanhf(0.7978845608f * (x + 0.044715f * (x * x * x))));
+        case INT8_ACT_GELU: {
+            // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u))
+            const float u = 0.7978845608f * (x + 0.044715f * (x * x * x));
+            return __fdividef(x, 1.0f + expf(-2.0f * u));
+        }
         case INT8_ACT_RELU: return x > 0.0f ? x : (x <= 0.0f ? 0.0f : x);  // a NaN stays one
         case INT8_ACT_GELU_ERF: return 0.5f * x * (1.0f + erff(x * 0.70710678118654752440f));
-        case INT8_ACT_SIGMOID: return 1.0f / (1.0f + expf(-x));
-        default: return x / (1.0f + expf(-x));
+        case INT8_ACT_SIGMOID: return __fdividef(1.0f, 1.0f + expf(-x));
+        default: return __fdividef(x, 1.0f + expf(-x));
     }
 }
 
@@ -39,6 +46,85 @@ struct Int8Product {
     int n_out;         // columns of y: n, or, gated, the pairs that are real
     long long ldy;
     unsigned int* status;
+};
+
+// Where a tile of a product lies: its weight tile, its expert, its tokens.
+struct Int8Tile {
+    int tn, e, row0, toks;
+};
+// The tiles of all experts as one list: of up to `bn` tokens of one expert each, the tokens of a weight tile one after the other.
+inline constexpr size_t int8_list_bytes(int experts) { return experts > 1 ? 8 * (size_t)(experts + 1) + 128 : 0; }
+struct Int8TileList {
+    const int* start;    // shared memory: tiles before each expert's, experts + 1 of them (null: one matrix)
+    const int* offsets;  // shared memory
+    int experts, rows, bn, tiles_n, ntiles, at;
+
+    // by all threads of a CTA; `shared`: int8_list_bytes
+    template <int THREADS> __device__ __forceinline__ void build(const Int8Product& p, int bn_, int tiles_n_, int* shared) {
+        start = offsets = nullptr;
+        experts = p.experts;
+        rows = p.rows;
+        bn = bn_;
+        tiles_n = tiles_n_;
+        at = 0;
+        if (p.offsets != nullptr) grid_dependency_wait();  // where the experts' rows begin is the work of a launch before
+        if (experts == 1) {
+            if (p.offsets != nullptr) rows = min(max(p.offsets[1], 0), p.rows);
+            ntiles = (rows + bn - 1) / bn * tiles_n;
+            return;
+        }
+        const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+        int *scan = shared, *off = shared + 32, *st = off + experts + 1;
+        for (int i = tid; i <= experts; i += THREADS) off[i] = min(max(p.offsets[i], 0), p.rows);
+        __syncthreads();
+        const int per = (experts + THREADS - 1) / THREADS, e0 = tid * per, e1 = min(e0 + per, experts);
+        int sum = 0;
+        for (int e = e0; e < e1; ++e) sum += (max(off[e + 1] - off[e], 0) + bn - 1) / bn * tiles_n;
+        int upto = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += v;
+        }
+        if (lane == 31) scan[warp] = upto;
+        __syncthreads();
+        int before = upto - sum;
+        for (int w = 0; w < warp; ++w) before += scan[w];
+        for (int e = e0; e < e1; ++e) {
+            st[e] = before;
+            before += (max(off[e + 1] - off[e], 0) + bn - 1) / bn * tiles_n;
+            if (e == experts - 1) st[experts] = before;
+        }
+        __syncthreads();
+        start = st;
+        offsets = off;
+        ntiles = st[experts];
+    }
+    // by whole warps, with tiles that do not fall
+    __device__ __forceinline__ Int8Tile find(int tile, int lane) {
+        Int8Tile t;
+        int first = 0, count = rows;
+        t.e = 0;
+        if (start != nullptr) {
+            for (;; at += 32) {
+                const int i = at + lane + 1;
+                const unsigned above = __ballot_sync(0xffffffffu, i > experts || start[i] > tile);
+                if (above != 0) {
+                    t.e = at + __ffs(above) - 1;
+                    break;
+                }
+            }
+            tile -= start[t.e];
+            first = offsets[t.e];
+            count = offsets[t.e + 1] - first;
+        }
+        const int tiles_m = (count + bn - 1) / bn;
+        t.tn = tile / tiles_m;
+        const int tm = tile - t.tn * tiles_m;
+        t.row0 = first + tm * bn;
+        t.toks = min(bn, count - tm * bn);
+        return t;
+    }
 };
 
 template <typename Kern, typename... Args>
@@ -61,9 +147,10 @@ cudaError_t int8_quantize_rows(int elem, const void* x, long long ldx, int8_t* q
                                const int* position, int topk, const int* row_limit, cudaStream_t s, bool dependent);
 cudaError_t int8_dequantize_rows(int elem, const int8_t* q, long long ldq, const float* scales, void* out, long long rows, int k, cudaStream_t s);
 // int8_rows.cu
+bool int8_rows_pays(const Int8Product& p);
 cudaError_t int8_product_rows(int elem, const Int8Product& p, cudaStream_t s, bool dependent);
 // int8_pair.cu
-bool int8_pair_pays(const Int8Product& p);
+bool int8_pair_ready();
 int int8_product_pair(int elem, const Int8Product& p, cudaStream_t s, bool dependent);
 // token_routing.cu
 cudaError_t route_sort(const void* ids, bool wide, int slots, int experts, int* order, int* offsets, int* position, cudaStream_t s);

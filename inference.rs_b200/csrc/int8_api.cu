@@ -28,8 +28,8 @@ static int check_routing(long long tokens, int topk, int experts) {
 }
 
 static int int8_product(int elem, const Int8Product& p, cudaStream_t s, bool dependent) {
-    if (int8_pair_pays(p)) return int8_product_pair(elem, p, s, dependent);
-    return cuda_result(int8_product_rows(elem, p, s, dependent));
+    if (int8_rows_pays(p) || !int8_pair_ready()) return cuda_result(int8_product_rows(elem, p, s, dependent));
+    return int8_product_pair(elem, p, s, dependent);
 }
 
 // What the experts' layer keeps between its launches, one region after the other, each on a 256-byte boundary.

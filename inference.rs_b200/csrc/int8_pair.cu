@@ -19,9 +19,12 @@ namespace b200q {
 constexpr int I8P_ROWS = 128;      // weight rows of one CTA = TMEM lanes
 constexpr int I8P_TOKENS = 256;    // tokens of a tile at most = TMEM columns of one accumulator
 constexpr int I8P_BK = 128;        // k per stage: one 128-byte swizzled row
-constexpr int I8P_MAX_STAGES = 12;
+constexpr int I8P_SUB = 2;         // such pieces per stage: the hand-over of a stage from TMA to tensor core and back takes as long as a
+                                   // small tile's products of 128 k (16 tokens, 16384 k: 345 cycles per 128 k with one, 275 with two)
+constexpr int I8P_MAX_STAGES = 6;
 constexpr int I8P_A_BYTES = I8P_ROWS * I8P_BK;
-constexpr int I8P_THREADS = 256;   // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warps 4-7 epilogue
+constexpr int I8P_THREADS = 384;   // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warps 4-11 epilogue
+constexpr int I8P_EPILOGUE = 8;    // warps: two to a quarter of the TMEM lanes, taking its columns 32 at a time in turn
 constexpr int I8P_TMEM_COLS = 512;
 
 struct Int8PairParams {
@@ -34,49 +37,14 @@ struct Int8PairBarriers {
     uint64_t full[I8P_MAX_STAGES], empty[I8P_MAX_STAGES];
     uint64_t tmem_full[2], tmem_empty[2];
     uint32_t tmem_base;
-    int scan[I8P_THREADS / 32];
 };
 static size_t i8p_smem(int stages, int bn, int experts) {
-    return 1024 + (size_t)stages * (I8P_A_BYTES + bn / 2 * I8P_BK) + sizeof(Int8PairBarriers) + (experts > 1 ? 8 * (size_t)(experts + 1) : 0);
+    return 1024 + (size_t)stages * I8P_SUB * (I8P_A_BYTES + bn / 2 * I8P_BK) + sizeof(Int8PairBarriers) + int8_list_bytes(experts);
 }
 
-// Where a tile lies: its weight tile, its expert, its tokens.
-struct Int8Tile {
-    int tn, e, row0, toks;
-};
-struct Int8TileList {
-    const int* start;    // shared memory: tiles before each expert's, experts + 1 of them (null: one matrix)
-    const int* offsets;  // shared memory
-    int experts, rows, bn, tiles_n, ntiles, at;
-    // called by whole warps, with tiles that do not fall
-    __device__ __forceinline__ Int8Tile find(int tile, int lane) {
-        Int8Tile t;
-        int first = 0, count = rows;
-        t.e = 0;
-        if (start != nullptr) {
-            for (;; at += 32) {
-                const int i = at + lane + 1;
-                const unsigned above = __ballot_sync(0xffffffffu, i > experts || start[i] > tile);
-                if (above != 0) {
-                    t.e = at + __ffs(above) - 1;
-                    break;
-                }
-            }
-            tile -= start[t.e];
-            first = offsets[t.e];
-            count = offsets[t.e + 1] - first;
-        }
-        const int tiles_m = (count + bn - 1) / bn;
-        t.tn = tile / tiles_m;
-        const int tm = tile - t.tn * tiles_m;
-        t.row0 = first + tm * bn;
-        t.toks = min(bn, count - tm * bn);
-        return t;
-    }
-};
 __device__ __forceinline__ int tile_columns(int toks) { return (toks + 31) & ~31; }  // N of the instruction
 
-template <typename OutT, bool GATED>
+template <typename OutT, int ACT>  // ACT: INT8_ACT_NONE, or the activation of a gated product
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, const Int8PairParams pp) {
     extern __shared__ uint8_t i8p_smem_raw[];
@@ -84,14 +52,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     const Int8Product& p = pp.p;
     uint8_t* a_stages = smem;
     const int stages = pp.stages, half = pp.bn / 2, b_bytes = half * I8P_BK;  // bytes: a multiple of 1024
-    uint8_t* b_stages = smem + stages * I8P_A_BYTES;
-    Int8PairBarriers* bars = reinterpret_cast<Int8PairBarriers*>(b_stages + stages * b_bytes);
+    uint8_t* b_stages = smem + stages * I8P_SUB * I8P_A_BYTES;
+    Int8PairBarriers* bars = reinterpret_cast<Int8PairBarriers*>(b_stages + stages * I8P_SUB * b_bytes);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_ctarank();
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
     const int nkb = (p.k + I8P_BK - 1) / I8P_BK;
-    const uint32_t stage_bytes = 2u * (I8P_A_BYTES + (uint32_t)b_bytes);  // both CTAs' operands of a stage
+    const uint32_t piece_bytes = 2u * (I8P_A_BYTES + (uint32_t)b_bytes);  // both CTAs' operands of a piece
+    const int nst = (nkb + I8P_SUB - 1) / I8P_SUB;
+    const auto pieces = [&](int st) { return min(I8P_SUB, nkb - st * I8P_SUB); };
 
     if (tid == 0) {
         for (int s = 0; s < stages; ++s) {
@@ -100,72 +70,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&bars->tmem_full[s], 1);
-            mbar_init(&bars->tmem_empty[s], 8);  // four epilogue warps of each CTA
+            mbar_init(&bars->tmem_empty[s], 2 * I8P_EPILOGUE);
         }
         mbar_init_fence();
     }
     if (warp == 2) tmem_alloc_pair(&bars->tmem_base, I8P_TMEM_COLS);
-    grid_dependency_wait();  // the rows, and where the experts' begin, are the work of the launch before
-    grid_launch_dependents();
-
-    Int8TileList list{nullptr, nullptr, p.experts, p.rows, pp.bn, pp.tiles_n, 0, 0};
-    if (p.experts > 1) {
-        int* offsets = reinterpret_cast<int*>(bars + 1);
-        int* start = offsets + p.experts + 1;
-        for (int i = tid; i <= p.experts; i += I8P_THREADS) offsets[i] = min(max(p.offsets[i], 0), p.rows);
-        __syncthreads();
-        const int per = (p.experts + I8P_THREADS - 1) / I8P_THREADS, e0 = tid * per, e1 = min(e0 + per, p.experts);
-        int sum = 0;
-        for (int e = e0; e < e1; ++e) sum += (max(offsets[e + 1] - offsets[e], 0) + pp.bn - 1) / pp.bn * pp.tiles_n;
-        int upto = sum;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += v;
-        }
-        if (lane == 31) bars->scan[warp] = upto;
-        __syncthreads();
-        int before = upto - sum;
-        for (int w = 0; w < warp; ++w) before += bars->scan[w];
-        for (int e = e0; e < e1; ++e) {
-            start[e] = before;
-            before += (max(offsets[e + 1] - offsets[e], 0) + pp.bn - 1) / pp.bn * pp.tiles_n;
-            if (e == p.experts - 1) start[p.experts] = before;
-        }
-        __syncthreads();
-        list.start = start;
-        list.offsets = offsets;
-        list.ntiles = start[p.experts];
-    } else {
-        if (p.offsets != nullptr) list.rows = min(max(p.offsets[1], 0), p.rows);
-        list.ntiles = (list.rows + pp.bn - 1) / pp.bn * pp.tiles_n;
-    }
+    Int8TileList list{};
+    list.build<I8P_THREADS>(p, pp.bn, pp.tiles_n, reinterpret_cast<int*>(bars + 1));
     tc_fence_before();
     __syncthreads();
     cluster_sync();  // the other CTA's barriers exist before anything arrives at them
     tc_fence_after();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
     const int ntiles = list.ntiles;
-
     if (warp == 0) {
         // ---------------- TMA: this CTA's 128 weight rows and half of the tokens; the leader's barrier counts both CTAs' bytes ----
         int s = 0, g = 0;
         uint32_t ph = 1;
         bool ok = true;
         const uint32_t full0 = map_to_rank(&bars->full[0], 0);
+        // The weights are no launch's work: the first stages' are on their way before the rows are there.
+        int early = 0;
+        if (p.offsets == nullptr && pair < ntiles) {
+            const Int8Tile t = list.find(pair, lane);
+            const int row = t.e * p.n + t.tn * 2 * I8P_ROWS + (int)rank * I8P_ROWS;
+            early = min(stages, nst);
+            if (elect_one()) {
+                for (int i = 0; i < early; ++i) {
+                    if (rank == 0) mbar_arrive_expect_tx(&bars->full[i], pieces(i) * piece_bytes);
+                    for (int j = 0; j < pieces(i); ++j)
+                        tma_load_2d_pair(a_stages + (size_t)(i * I8P_SUB + j) * I8P_A_BYTES, &tmap_w, (i * I8P_SUB + j) * I8P_BK, row, full0 + 8u * i);
+                }
+            }
+            __syncwarp();
+        }
+        grid_dependency_wait();
+        grid_launch_dependents();
         for (int tile = pair; tile < ntiles && ok; tile += npairs) {
             const Int8Tile t = list.find(tile, lane);
             const int row = t.e * p.n + t.tn * 2 * I8P_ROWS + (int)rank * I8P_ROWS, token = t.row0 + (int)rank * (tile_columns(t.toks) / 2);
-            for (int kb = 0; kb < nkb; ++kb, ++g) {
+            for (int kb = 0; kb < nst; ++kb, ++g) {
                 ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars->empty[s], ph));
                 if (!ok) {
                     if (lane == 0) record_failure(p.status, STATUS_WAIT_EMPTY_TIMEOUT, g);
                     break;
                 }
                 if (elect_one()) {
-                    if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], stage_bytes);
-                    tma_load_2d_pair(a_stages + (size_t)s * I8P_A_BYTES, &tmap_w, kb * I8P_BK, row, full0 + 8u * s);
-                    tma_load_2d_pair(b_stages + (size_t)s * b_bytes, &tmap_x, kb * I8P_BK, token, full0 + 8u * s);
+                    if (g >= early && rank == 0) mbar_arrive_expect_tx(&bars->full[s], pieces(kb) * piece_bytes);
+                    for (int j = 0; j < pieces(kb); ++j) {
+                        const int at = s * I8P_SUB + j, k = (kb * I8P_SUB + j) * I8P_BK;
+                        if (g >= early) tma_load_2d_pair(a_stages + (size_t)at * I8P_A_BYTES, &tmap_w, k, row, full0 + 8u * s);
+                        tma_load_2d_pair(b_stages + (size_t)at * b_bytes, &tmap_x, k, token, full0 + 8u * s);
+                    }
                 }
                 __syncwarp();
                 if (++s == stages) {
@@ -202,19 +158,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
                 }
                 tc_fence_after();
                 const uint32_t d = tmem_base + buf * I8P_TOKENS;
-                for (int kb = 0; kb < nkb; ++kb) {
+                for (int kb = 0; kb < nst; ++kb) {
                     ok = __all_sync(0xffffffffu, mbar_wait_bounded(&bars->full[s], ph));
                     if (!ok) {
                         if (lane == 0) record_failure(p.status, STATUS_WAIT_FULL_TIMEOUT, kb);
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t da = da0 + (uint64_t)(s * (I8P_A_BYTES >> 4)), db = db0 + (uint64_t)(s * (b_bytes >> 4));
+                    const uint64_t da = da0 + (uint64_t)(s * I8P_SUB * (I8P_A_BYTES >> 4)), db = db0 + (uint64_t)(s * I8P_SUB * (b_bytes >> 4));
                     if (elect_one()) {
+                        for (int j = 0; j < pieces(kb); ++j) {
+                            const uint64_t dja = da + (uint64_t)(j * (I8P_A_BYTES >> 4)), djb = db + (uint64_t)(j * (b_bytes >> 4));
 #pragma unroll
-                        for (int k = 0; k < I8P_BK / 32; ++k) tc_mma_i8_pair(d, da + 2 * k, db + 2 * k, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                            for (int k = 0; k < I8P_BK / 32; ++k) tc_mma_i8_pair(d, dja + 2 * k, djb + 2 * k, idesc, (kb > 0 || j > 0 || k > 0) ? 1u : 0u);
+                        }
                         tc_commit_pair(&bars->empty[s]);  // frees the stage in both CTAs when these MMAs have read it
-                        if (kb == nkb - 1) tc_commit_pair(&bars->tmem_full[buf]);
+                        if (kb == nst - 1) tc_commit_pair(&bars->tmem_full[buf]);
                     }
                     __syncwarp();
                     if (++s == stages) {
@@ -226,7 +185,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
         }
     } else if (warp >= 4) {
         // ---------------- epilogue: thread = weight row, 32 tokens at a time; a warp's store is 32 neighbouring outputs ----------------
-        const int quarter = warp & 3;
+        const int quarter = warp & 3, turn = (warp - 4) >> 2;
+        grid_dependency_wait();
         bool ok = true;
         int ti = 0;
         for (int tile = pair; tile < ntiles; tile += npairs, ++ti) {
@@ -243,29 +203,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
             tc_fence_after();
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * I8P_TOKENS;
             OutT* y = static_cast<OutT*>(p.y) + (long long)t.row0 * p.ldy;
-            for (int c = 0; c < t.toks; c += 32) {
+            for (int c = 32 * turn; c < t.toks; c += 32 * (I8P_EPILOGUE / 4)) {
                 const float xs = c + lane < t.toks ? p.xs[t.row0 + c + lane] : 0.0f;
                 uint32_t acc[32];
                 tmem_ld_32x32(taddr + c, acc);
                 float v[32];
 #pragma unroll
                 for (int j = 0; j < 32; ++j) v[j] = (float)(int)acc[j] * __shfl_sync(0xffffffffu, xs, j) * ws;
-                if constexpr (!GATED) {
-                    if (n < p.n) {
+                OutT* dst = y + c * p.ldy;
+                if constexpr (ACT == INT8_ACT_NONE) {
+                    dst += n;
+                    const int toks = n < p.n ? t.toks - c : 0;
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (c + j < t.toks) y[(long long)(c + j) * p.ldy + n] = from_float<OutT>(v[j]);
+                    for (int j = 0; j < 32; ++j) {
+                        if (j < toks) *dst = from_float<OutT>(v[j]);
+                        dst += p.ldy;
                     }
                 } else {
                     // rows 8.. of 16 hold up, the others gate: the lane of a gate row takes tokens 0..15, that of its up row 16..31
                     const bool is_up = (lane & 8) != 0;
-                    const int col = (n >> 4) * 8 + (n & 7);
+                    const int col = (n >> 4) * 8 + (n & 7), from = is_up ? 16 : 0;
+                    const int toks = col < p.n_out ? t.toks - c - from : 0;
+                    dst += from * p.ldy + col;
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const float other = __shfl_xor_sync(0xffffffffu, is_up ? v[j] : v[16 + j], 8);
                         const float gate = is_up ? other : v[j], up = is_up ? v[16 + j] : other;
-                        const int tok = c + (is_up ? 16 + j : j);
-                        if (col < p.n_out && tok < t.toks) y[(long long)tok * p.ldy + col] = from_float<OutT>(int8_activate(gate, p.act) * up);
+                        if (j < toks) *dst = from_float<OutT>(int8_activate(gate, ACT) * up);
+                        dst += p.ldy;
                     }
                 }
             }
@@ -307,7 +272,7 @@ static int int8_token_tile(const Int8Product& p, int tiles_n) {
     return best_bn;
 }
 
-template <typename OutT, bool GATED> static int pair_t(const Int8Product& p, cudaStream_t s, bool dependent) {
+template <typename OutT, int ACT> static int pair_t(const Int8Product& p, cudaStream_t s, bool dependent) {
     Int8PairParams pp{};
     pp.p = p;
     pp.tiles_n = (p.n + 2 * I8P_ROWS - 1) / (2 * I8P_ROWS);
@@ -330,7 +295,7 @@ template <typename OutT, bool GATED> static int pair_t(const Int8Product& p, cud
                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != CUDA_SUCCESS)
             return set_error(B200Q_ERR_INVALID, "no tensor map for the activations");
     }
-    constexpr auto kernel = int8_pair_kernel<OutT, GATED>;
+    constexpr auto kernel = int8_pair_kernel<OutT, ACT>;
     cudaError_t e = allow_full_smem<kernel>();
     if (e == cudaSuccess) {
         const int pairs = runtime_info().sm_count / 2;
@@ -342,10 +307,17 @@ template <typename OutT, bool GATED> static int pair_t(const Int8Product& p, cud
     return e == cudaSuccess ? B200Q_OK : set_error((int)e, cudaGetErrorString(e));
 }
 template <typename OutT> static int pair_out(const Int8Product& p, cudaStream_t s, bool dependent) {
-    return p.act == INT8_ACT_NONE ? pair_t<OutT, false>(p, s, dependent) : pair_t<OutT, true>(p, s, dependent);
+    switch (p.act) {
+        case INT8_ACT_NONE: return pair_t<OutT, INT8_ACT_NONE>(p, s, dependent);
+        case INT8_ACT_GELU: return pair_t<OutT, INT8_ACT_GELU>(p, s, dependent);
+        case INT8_ACT_RELU: return pair_t<OutT, INT8_ACT_RELU>(p, s, dependent);
+        case INT8_ACT_GELU_ERF: return pair_t<OutT, INT8_ACT_GELU_ERF>(p, s, dependent);
+        case INT8_ACT_SIGMOID: return pair_t<OutT, INT8_ACT_SIGMOID>(p, s, dependent);
+        default: return pair_t<OutT, INT8_ACT_SILU>(p, s, dependent);
+    }
 }
 
-bool int8_pair_pays(const Int8Product& p) { return encode_tiled_fn() != nullptr && p.rows > 64 * p.experts; }
+bool int8_pair_ready() { return encode_tiled_fn() != nullptr; }
 
 int int8_product_pair(int elem, const Int8Product& p, cudaStream_t s, bool dependent) {
     if (elem == ELEM_F32) return pair_out<float>(p, s, dependent);

@@ -5,11 +5,13 @@
 // (Values so small that s is no normal float, under 1.5e-36, may have quotients above 127: they count as 127.)
 //
 // The quotient is never formed by division: t = x * (1 / s) is off by less than 2e-5, so round(t) is the integer unless t lies that
-// close to a half, and there the remainder x - q s, which one fused multiply-add gives exactly (|q| <= 127 and s have 31 bits together,
-// and the remainder is a multiple of half the last place of s), decides. A row with an infinity or a NaN in it has a NaN for a scale and
+// close to a half, and there the remainder x - q s, which one fused multiply-add gives exactly (it is a multiple of half the last place
+// of s, and not much more than s / 2), decides. A row with an infinity or a NaN in it has a NaN for a scale and
 // zeros for integers: its products are NaN, as they would be in floating point, and no other row's.
 //
 // Bound by HBM: a row is read once, held in registers between the maximum and the rounding, and written as one byte a value.
+#include <type_traits>
+
 #include "int8.cuh"
 
 namespace b200q {
@@ -27,9 +29,12 @@ struct QuantizeRows {
     const int* row_limit;  // rows from here on are left alone (null: none)
 };
 
+constexpr float ROUND = 12582912.0f;  // 1.5 * 2^23: v + ROUND has the integer next to v in its low bits
+
 struct RowScale {
-    float s;    // as stored
-    float sn, inv, pre, near_half;  // x * pre / sn is the same quotient, with sn far from the smallest floats
+    float s;          // as stored
+    float sn, inv;    // x * pre / sn is the same quotient, with sn far from the smallest floats; inv 0: the integers are zeros
+    float pre, half;  // half of sn
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
     RowScale r;
@@ -38,27 +43,48 @@ __device__ __forceinline__ RowScale row_scale(uint32_t amax_bits) {
     r.pre = r.s < 1e-30f ? 18446744073709551616.0f : 1.0f;  // 2^64
     r.sn = r.s * r.pre;
     r.inv = finite && r.s > 0.0f ? 1.0f / r.sn : 0.0f;
-    r.near_half = 0.4999f * r.sn;
+    r.half = 0.5f * r.sn;
     return r;
 }
-__device__ __noinline__ float nearest_quotient(float x, float qf, float sn) {
-    const float rem = fmaf(-qf, sn, x), half = 0.5f * sn;
-    const bool odd = ((int)qf & 1) != 0;
-    if (rem > half || (rem == half && odd)) return qf + 1.0f;
-    if (rem < -half || (rem == -half && odd)) return qf - 1.0f;
-    return qf;
+// Four values, one byte each, where a value may lie exactly on a half, or the scale is among the smallest floats.
+__device__ __noinline__ uint32_t quantize_four_carefully(float a, float b, float c, float d, float sn, float inv, float pre) {
+    const float v[4] = {a, b, c, d}, half = 0.5f * sn;
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = v[i] * pre;
+        float q = fmaf(x, inv, ROUND) - ROUND;
+        const float rem = fmaf(-q, sn, x);
+        const bool odd = ((int)q & 1) != 0;
+        if (rem > half || (rem == half && odd)) q += 1.0f;
+        else if (rem < -half || (rem == -half && odd)) q -= 1.0f;
+        w |= ((uint32_t)(int)fminf(fmaxf(q, -127.0f), 127.0f) & 0xffu) << (8 * i);
+    }
+    return w;
 }
-__device__ __forceinline__ uint32_t quantize_one(float x, const RowScale& r) {
-    if (r.inv == 0.0f) return 0u;  // a row of zeros, or with a value that is not finite
-    const float xs = x * r.pre;
-    float qf = fmaf(xs, r.inv, 12582912.0f) - 12582912.0f;
-    if (fabsf(fmaf(-qf, r.sn, xs)) > r.near_half) qf = nearest_quotient(xs, qf, r.sn);
-    if (r.pre != 1.0f) qf = fminf(fmaxf(qf, -127.0f), 127.0f);
-    return (uint32_t)(int)qf & 0xffu;
+// The remainder settles every value without a branch: one bf16 value in some hundred has a quotient within a rounding of s of a half (127
+// times one 8-bit mantissa by another), so a way out of line for them was taken by every other warp and cost as much as all the rest.
+// HALVES: a value can lie on a half exactly without s being a power of two, for which the rounding of x * (1 / s) is right as it is. Not
+// so for bf16: half an odd multiple of s has 8 bits only where s has one.
+template <bool HALVES> __device__ __forceinline__ uint32_t quantize_four(float a, float b, float c, float d, const RowScale& r) {
+    if (r.pre != 1.0f) return quantize_four_carefully(a, b, c, d, r.sn, r.inv, r.pre);
+    const float v[4] = {a, b, c, d};
+    float t[4];
+    bool on_half = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        t[i] = fmaf(v[i], r.inv, ROUND);
+        const float rem = fmaf(ROUND - t[i], r.sn, v[i]);
+        if constexpr (HALVES) on_half |= fabsf(rem) == r.half;
+        if (fabsf(rem) > r.half) t[i] += copysignf(1.0f, rem);
+    }
+    if (HALVES && on_half) return quantize_four_carefully(a, b, c, d, r.sn, r.inv, 1.0f);
+    return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
 }
 
 // Eight values of a row as they lie in memory. Plain loads: what they read may be the work of the launch before, which this one waited
-// for after it had started.
+// for after it had started. `top` is the largest magnitude as a bit pattern of the type: patterns without their sign are in the order of
+// the values, with infinities and NaN above all.
 template <typename T> struct Eight;
 template <> struct Eight<float> {
     float4 a, b;
@@ -67,19 +93,31 @@ template <> struct Eight<float> {
         b = *(reinterpret_cast<const float4*>(p) + 1);
     }
     __device__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
-    __device__ void get(float (&v)[8]) const {
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    static __device__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+    __device__ uint32_t top(uint32_t m) const {
+        m = max(m, max(max(abs_bits(a.x), abs_bits(a.y)), max(abs_bits(a.z), abs_bits(a.w))));
+        return max(m, max(max(abs_bits(b.x), abs_bits(b.y)), max(abs_bits(b.z), abs_bits(b.w))));
     }
+    static __device__ uint32_t float_bits(uint32_t top) { return top; }
+    __device__ uint2 quantize(const RowScale& r) const { return make_uint2(quantize_four<true>(a.x, a.y, a.z, a.w, r), quantize_four<true>(b.x, b.y, b.z, b.w, r)); }
 };
 template <typename T> struct Eight {
     uint4 a;
     __device__ void load(const T* p) { a = *reinterpret_cast<const uint4*>(p); }
     __device__ void zero() { a = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ void get(float (&v)[8]) const {
+    __device__ uint32_t top(uint32_t m) const {  // two patterns side by side
+        const uint32_t lo = __vmaxu2(a.x & 0x7fff7fffu, a.y & 0x7fff7fffu), hi = __vmaxu2(a.z & 0x7fff7fffu, a.w & 0x7fff7fffu);
+        return __vmaxu2(m, __vmaxu2(lo, hi));
+    }
+    static __device__ uint32_t float_bits(uint32_t top) {
+        const unsigned short t = (unsigned short)max(top & 0xffffu, top >> 16);
+        return __float_as_uint(to_float<T>(*reinterpret_cast<const T*>(&t)));
+    }
+    static constexpr bool HALVES = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value;
+    __device__ uint2 quantize(const RowScale& r) const {
         const T* e = reinterpret_cast<const T*>(&a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_float<T>(e[i]);
+        return make_uint2(quantize_four<HALVES>(to_float<T>(e[0]), to_float<T>(e[1]), to_float<T>(e[2]), to_float<T>(e[3]), r),
+                          quantize_four<HALVES>(to_float<T>(e[4]), to_float<T>(e[5]), to_float<T>(e[6]), to_float<T>(e[7]), r));
     }
 };
 
@@ -103,49 +141,67 @@ __device__ __forceinline__ void store_scale(const QuantizeRows& p, long long row
     }
 }
 
-// One CTA per row, eight values per thread and step.
-template <typename T, int STEPS> __global__ void __launch_bounds__(1024) int8_quantize_kernel(const QuantizeRows p) {
-    grid_dependency_wait();
-    grid_launch_dependents();
-    const long long row = blockIdx.x;
-    if (p.row_limit != nullptr && row >= *p.row_limit) return;
-    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    const int step = blockDim.x * 8, first = threadIdx.x * 8;
+// `size` threads (a warp or a CTA) and their share of a row: eight values per thread and step.
+template <typename T, int STEPS> struct RowPart {
     Eight<T> held[STEPS];
-    uint32_t amax = 0;
+    __device__ __forceinline__ void load(const QuantizeRows& p, long long row, int rank, int size) {
+        const T* x = static_cast<const T*>(p.x) + row * p.ldx;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        if (first + i * step < p.k) held[i].load(x + first + i * step);
-        else held[i].zero();
+        for (int i = 0; i < STEPS; ++i) {
+            const int c = 8 * (rank + i * size);
+            if (c < p.k) held[i].load(x + c);
+            else held[i].zero();
+        }
     }
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        float v[8];
-        held[i].get(v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max(amax, __float_as_uint(v[j]) & 0x7fffffffu);
+        for (int i = 0; i < STEPS; ++i) m = held[i].top(m);
+        return Eight<T>::float_bits(m);
     }
-    const RowScale r = row_scale(block_max(amax));
-    if (threadIdx.x == 0) store_scale(p, row, r.s);
-    const int kp = (p.k + 15) & ~15;
+    __device__ __forceinline__ void store(const QuantizeRows& p, long long row, const RowScale& r, int rank, int size) const {
+        const int kp = (p.k + 15) & ~15;
+        if (rank == 0) store_scale(p, row, r.s);
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-        const int c = first + i * step;
-        if (c >= kp) break;
-        float v[8];
-        held[i].get(v);
-        uint32_t w[2] = {0u, 0u};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j >> 2] |= quantize_one(v[j], r) << (8 * (j & 3));
-        if (p.position == nullptr) {
-            *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = make_uint2(w[0], w[1]);
-        } else {
-            for (int j = 0; j < p.topk; ++j) {
-                const int to = p.position[row * p.topk + j];
-                if (to >= 0) *reinterpret_cast<uint2*>(p.q + (long long)to * p.ldq + c) = make_uint2(w[0], w[1]);
+        for (int i = 0; i < STEPS; ++i) {
+            const int c = 8 * (rank + i * size);
+            if (c >= kp) break;
+            const uint2 w = r.inv != 0.0f ? held[i].quantize(r) : make_uint2(0u, 0u);
+            if (p.position == nullptr) {
+                *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = w;
+            } else {
+                for (int j = 0; j < p.topk; ++j) {
+                    const int to = p.position[row * p.topk + j];
+                    if (to >= 0) *reinterpret_cast<uint2*>(p.q + (long long)to * p.ldq + c) = w;
+                }
             }
         }
     }
+};
+__device__ __forceinline__ long long row_count(const QuantizeRows& p) {
+    return p.row_limit != nullptr ? min((long long)max(*p.row_limit, 0), p.rows) : p.rows;
+}
+
+// A CTA per row.
+template <typename T, int STEPS, int MAX_THREADS> __global__ void __launch_bounds__(MAX_THREADS) int8_quantize_kernel(const QuantizeRows p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const long long row = blockIdx.x;
+    if (row >= row_count(p)) return;
+    RowPart<T, STEPS> part;
+    part.load(p, row, threadIdx.x, blockDim.x);
+    part.store(p, row, row_scale(block_max(part.top())), threadIdx.x, blockDim.x);
+}
+// A warp per row, rows of up to 1024 values: a CTA for each such row would cost its start, about a nanosecond.
+template <typename T> __global__ void __launch_bounds__(256) int8_quantize_short_kernel(const QuantizeRows p) {
+    grid_dependency_wait();
+    grid_launch_dependents();
+    const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= row_count(p)) return;
+    RowPart<T, 4> part;
+    part.load(p, row, lane, 32);
+    part.store(p, row, row_scale(__reduce_max_sync(0xffffffffu, part.top())), lane, 32);
 }
 
 // Any width, any alignment of x: a value at a time, the row read twice.
@@ -161,10 +217,10 @@ template <typename T> __global__ void __launch_bounds__(256) int8_quantize_plain
     if (threadIdx.x == 0) store_scale(p, row, r.s);
     const int kp = (p.k + 15) & ~15;
     for (int c = 4 * threadIdx.x; c < kp; c += 1024) {
-        uint32_t w = 0;
+        float v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (c + j < p.k) w |= quantize_one(to_float<T>(x[c + j]), r) << (8 * j);
+        for (int j = 0; j < 4; ++j) v[j] = c + j < p.k ? to_float<T>(x[c + j]) : 0.0f;
+        const uint32_t w = r.inv != 0.0f ? quantize_four<true>(v[0], v[1], v[2], v[3], r) : 0u;
         if (p.position == nullptr) {
             *reinterpret_cast<uint32_t*>(p.q + row * p.ldq + c) = w;
         } else {
@@ -178,12 +234,15 @@ template <typename T> __global__ void __launch_bounds__(256) int8_quantize_plain
 
 template <typename T> static cudaError_t quantize_t(const QuantizeRows& p, cudaStream_t s, bool dependent) {
     const bool wide = p.k % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ldx * sizeof(T) % 16 == 0 && p.k <= 32768;
-    const dim3 grid((unsigned)p.rows, 1, 1);
-    if (!wide) return launch_kernel(int8_quantize_plain_kernel<T>, grid, 256, 0, s, dependent, p);
+    if (!wide) return launch_kernel(int8_quantize_plain_kernel<T>, dim3((unsigned)p.rows, 1, 1), 256, 0, s, dependent, p);
+    const long long sms = runtime_info().sm_count;
     const int eights = (p.k + 15) / 16 * 2, whole = (eights + 31) / 32 * 32;
-    // few rows: every thread one step, the shortest way; many: four steps, so that more loads are under way per thread
-    if (whole <= 1024 && (p.rows < 512 || whole <= 128)) return launch_kernel(int8_quantize_kernel<T, 1>, grid, (unsigned)whole, 0, s, dependent, p);
-    return launch_kernel(int8_quantize_kernel<T, 4>, grid, (unsigned)((eights + 127) / 128 * 32), 0, s, dependent, p);
+    // few rows: every thread as few steps as there can be, the shortest way
+    if (p.rows <= 2 * sms && whole <= 1024) return launch_kernel(int8_quantize_kernel<T, 1, 1024>, dim3((unsigned)p.rows, 1, 1), (unsigned)whole, 0, s, dependent, p);
+    if (p.k <= 1024) return launch_kernel(int8_quantize_short_kernel<T>, dim3((unsigned)((p.rows + 7) / 8), 1, 1), 256, 0, s, dependent, p);
+    const unsigned threads = (unsigned)((eights + 127) / 128 * 32);
+    if (threads <= 512) return launch_kernel(int8_quantize_kernel<T, 4, 512>, dim3((unsigned)p.rows, 1, 1), threads, 0, s, dependent, p);
+    return launch_kernel(int8_quantize_kernel<T, 4, 1024>, dim3((unsigned)p.rows, 1, 1), threads, 0, s, dependent, p);
 }
 
 cudaError_t int8_quantize_rows(int elem, const void* x, long long ldx, int8_t* q, long long ldq, float* scales, long long rows, int k,

@@ -1,9 +1,13 @@
-// Products of int8 rows on warp-level integer MMAs: a CTA owns 16 or 32 weight rows of one matrix and reads them once for up to 32
-// tokens, straight from global memory into MMA fragments. The warps of a CTA share the k range and add up through shared memory;
-// the sums are integers, so their order changes nothing.
+// Products of int8 rows on warp-level integer MMAs, for few tokens: what they cost is reading the weights, once, from HBM straight into MMA
+// fragments. One to eight warps of a CTA share a tile of 16 or 32 weight rows and 8 or 16 tokens, each a part of k, and add up through
+// shared memory; the sums are integers, so their order changes nothing.
 //
 // A lane loads 16 neighbouring bytes of a row: of the four words two make its part of one 32-k MMA and two that of the next. That takes
 // the k of a 64-byte piece in another order than they lie, the same one for weights and tokens, which a sum does not mind.
+//
+// The CTAs are persistent and a warp's loads run one batch of pieces ahead of its products, across the border from one tile to the next:
+// 64 KB on their way per SM all the time. (CTAs of one tile each, without that: 14336 x 4096 by one token 24.9 us against 13.4, 4096 x
+// 28672 24.1 against 20.3 of which HBM needs 18.)
 #include "int8.cuh"
 
 namespace b200q {
@@ -22,77 +26,171 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <typename OutT, int R, int NT>
-__global__ void __launch_bounds__(32 * I8R_WARPS) int8_rows_kernel(const Int8Product p) {
-    constexpr int ROWS = 16 * R, TOKENS = 8 * NT, PITCH = ROWS + 4;
-    __shared__ int sums[I8R_WARPS][TOKENS][PITCH];
-    grid_dependency_wait();
-    grid_launch_dependents();
-    const int e = blockIdx.y, row0 = blockIdx.x * ROWS;
-    const int first = p.offsets != nullptr ? max(p.offsets[e], 0) : 0, last = p.offsets != nullptr ? min(p.offsets[e + 1], p.rows) : p.rows;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int8_t* w[2 * R];
+// A lane's words of U pieces of 16 R weight rows and 8 NT tokens. Pieces from `steps` on, and lanes beyond the row's end, count as zeros.
+template <int R, int NT, int U, int WK> struct RowPieces {
+    uint4 a[U][2 * R], b[U][NT];
+    __device__ __forceinline__ void load_weights(const int8_t* const (&w)[2 * R], int step, int kp, int t) {
 #pragma unroll
-    for (int i = 0; i < 2 * R; ++i) w[i] = p.wq + ((long long)e * p.n + min(row0 + 8 * i + g, p.n - 1)) * p.ldw + 16 * t;
-    const int kp = (p.k + 15) & ~15, steps = (kp + I8R_STEP - 1) / I8R_STEP;
-    for (int tok0 = first; tok0 < last; tok0 += TOKENS) {
-        const int8_t* x[NT];
+        for (int u = 0; u < U; ++u) {
+            const int k0 = (step + u * WK) * I8R_STEP;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) x[j] = p.xq + (long long)min(tok0 + 8 * j + g, last - 1) * p.ldx + 16 * t;
-        int acc[R][NT][4] = {};
-#pragma unroll 2
-        for (int s = warp; s < steps; s += I8R_WARPS) {
-            const int k0 = s * I8R_STEP;
-            const bool in = k0 + 16 * t < kp;
-            uint4 a[2 * R], b[NT];
+            for (int i = 0; i < 2 * R; ++i) a[u][i] = k0 + 16 * t < kp ? ldg_stream(w[i] + k0) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    __device__ __forceinline__ void load_tokens(const int8_t* const (&x)[NT], int step, int kp, int t) {
 #pragma unroll
-            for (int i = 0; i < 2 * R; ++i) a[i] = in ? ldg_stream(w[i] + k0) : make_uint4(0u, 0u, 0u, 0u);
+        for (int u = 0; u < U; ++u) {
+            const int k0 = (step + u * WK) * I8R_STEP;
 #pragma unroll
-            for (int j = 0; j < NT; ++j) b[j] = in ? *reinterpret_cast<const uint4*>(x[j] + k0) : make_uint4(0u, 0u, 0u, 0u);
+            for (int j = 0; j < NT; ++j) b[u][j] = k0 + 16 * t < kp ? *reinterpret_cast<const uint4*>(x[j] + k0) : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    __device__ __forceinline__ void multiply(int (&acc)[R][NT][4]) const {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int i = 0; i < R; ++i)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    mma_s8(acc[i][j], a[2 * i].x, a[2 * i + 1].x, a[2 * i].y, a[2 * i + 1].y, b[j].x, b[j].y);
-                    mma_s8(acc[i][j], a[2 * i].z, a[2 * i + 1].z, a[2 * i].w, a[2 * i + 1].w, b[j].z, b[j].w);
+                    mma_s8(acc[i][j], a[u][2 * i].x, a[u][2 * i + 1].x, a[u][2 * i].y, a[u][2 * i + 1].y, b[u][j].x, b[u][j].y);
+                    mma_s8(acc[i][j], a[u][2 * i].z, a[u][2 * i + 1].z, a[u][2 * i].w, a[u][2 * i + 1].w, b[u][j].z, b[u][j].w);
                 }
+    }
+};
+
+template <typename OutT, int R, int NT, int U, int WK, int PER_SM>
+__global__ void __launch_bounds__(32 * I8R_WARPS, PER_SM) int8_rows_kernel(const Int8Product p) {
+    constexpr int ROWS = 16 * R, TOKENS = 8 * NT, PITCH = ROWS + 4, GROUPS = I8R_WARPS / WK;
+    __shared__ int sums[I8R_WARPS][TOKENS][PITCH];
+    extern __shared__ int lists[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int group = warp / WK, wk = warp % WK;
+    const int kp = (p.k + 15) & ~15, steps = (kp + I8R_STEP - 1) / I8R_STEP, batches = (steps + U * WK - 1) / (U * WK);
+    Int8TileList list{};
+    list.build<32 * I8R_WARPS>(p, TOKENS, (p.n + ROWS - 1) / ROWS, lists);
+    Int8TileList ahead = list;
+
+    // Loads run a batch ahead of the products, and on into the next tile.
+    RowPieces<R, NT, U, WK> now, next;
+    const int8_t *w[2 * R], *x[NT];
+    const int first_tile = blockIdx.x + gridDim.x * group, tile_step = gridDim.x * GROUPS;
+    int ahead_tile = first_tile, ahead_batch = 0;
+    const auto aim = [&] {
+        const Int8Tile at = ahead.find(ahead_tile, lane);
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i) w[i] = p.wq + ((long long)at.e * p.n + min(at.tn * ROWS + 8 * i + g, p.n - 1)) * p.ldw + 16 * t;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) x[j] = p.xq + (long long)(at.row0 + min(8 * j + g, at.toks - 1)) * p.ldx + 16 * t;
+    };
+    const auto advance = [&] {
+        if (++ahead_batch < batches) return;
+        ahead_batch = 0;
+        ahead_tile += tile_step;
+        if (ahead_tile < list.ntiles) aim();
+    };
+    const auto fill = [&](RowPieces<R, NT, U, WK>& pieces) {
+        if (ahead_tile >= list.ntiles) return;
+        pieces.load_weights(w, ahead_batch * U * WK + wk, kp, t);
+        pieces.load_tokens(x, ahead_batch * U * WK + wk, kp, t);
+        advance();
+    };
+    if (ahead_tile < list.ntiles) {
+        aim();
+        now.load_weights(w, wk, kp, t);  // the weights are no launch's work: on their way before the rows are there
+    }
+    grid_dependency_wait();
+    grid_launch_dependents();
+    if (ahead_tile < list.ntiles) {
+        now.load_tokens(x, wk, kp, t);
+        advance();
+    }
+    bool flip = false;
+    for (int tile = first_tile; tile < list.ntiles; tile += tile_step) {
+        int acc[R][NT][4] = {};
+        for (int b = 0; b < batches; ++b) {
+            if (!flip) {
+                fill(next);
+                now.multiply(acc);
+            } else {
+                fill(now);
+                next.multiply(acc);
+            }
+            flip = !flip;
         }
+        const Int8Tile at = list.find(tile, lane);
+        const int row0 = at.tn * ROWS;
+        const float* ws = p.ws + (long long)at.e * p.n + row0;
+        const float* xs = p.xs + at.row0;
+        OutT* y = static_cast<OutT*>(p.y) + (long long)at.row0 * p.ldy;
+        const auto put = [&](int tok, int r, int sum) {  // row r of the tile
+            if (row0 + r < p.n) y[tok * p.ldy + row0 + r] = from_float<OutT>((float)sum * xs[tok] * ws[r]);
+        };
+        const auto put_gated = [&](int tok, int r, int gate, int up) {  // r: the gate's row, up is 8 rows on
+            const int col = row0 / 2 + (r >> 4) * 8 + (r & 7);
+            if (col < p.n_out) y[tok * p.ldy + col] = from_float<OutT>(int8_activate((float)gate * xs[tok] * ws[r], p.act) * ((float)up * xs[tok] * ws[r + 8]));
+        };
 #pragma unroll
         for (int i = 0; i < R; ++i)
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) sums[warp][8 * j + 2 * t + (c & 1)][16 * i + g + 8 * (c >> 1)] = acc[i][j][c];
-        __syncthreads();
-        const int toks = min(TOKENS, last - tok0);
-        auto value = [&](int tok, int r) {
+        named_bar_sync(1 + group, 32 * WK);
+        const auto total = [&](int tok, int r) {
             int sum = 0;
 #pragma unroll
-            for (int v = 0; v < I8R_WARPS; ++v) sum += sums[v][tok][r];
-            return (float)sum * p.xs[tok0 + tok] * p.ws[(long long)e * p.n + row0 + r];
+            for (int v = 0; v < WK; ++v) sum += sums[group * WK + v][tok][r];
+            return sum;
         };
-        OutT* y = static_cast<OutT*>(p.y) + (long long)tok0 * p.ldy;
+        const int member = wk * 32 + lane;
         if (p.act == INT8_ACT_NONE) {
-            for (int i = threadIdx.x; i < toks * ROWS; i += 32 * I8R_WARPS) {
-                const int r = i % ROWS, tok = i / ROWS;
-                if (row0 + r < p.n) y[tok * p.ldy + row0 + r] = from_float<OutT>(value(tok, r));
-            }
+            for (int i = member; i < at.toks * ROWS; i += 32 * WK) put(i / ROWS, i % ROWS, total(i / ROWS, i % ROWS));
         } else {
-            for (int i = threadIdx.x; i < toks * ROWS / 2; i += 32 * I8R_WARPS) {
+            for (int i = member; i < at.toks * ROWS / 2; i += 32 * WK) {
                 const int c = i % (ROWS / 2), tok = i / (ROWS / 2), r = (c & ~7) * 2 + (c & 7);
-                if (row0 / 2 + c < p.n_out) y[tok * p.ldy + row0 / 2 + c] = from_float<OutT>(int8_activate(value(tok, r), p.act) * value(tok, r + 8));
+                put_gated(tok, r, total(tok, r), total(tok, r + 8));
             }
         }
-        __syncthreads();
+        named_bar_sync(1 + group, 32 * WK);
     }
 }
 
+template <typename OutT, int R, int NT, int U, int WK, int PER_SM> static cudaError_t rows_launch(const Int8Product& p, cudaStream_t s, bool dependent) {
+    // at most one group of tokens more per expert than the rows fill
+    const long long tiles = (long long)((p.n + 16 * R - 1) / (16 * R)) * ((p.rows + 8 * NT - 1) / (8 * NT) + p.experts - 1), fit = (long long)PER_SM * runtime_info().sm_count;
+    return launch_kernel(int8_rows_kernel<OutT, R, NT, U, WK, PER_SM>, dim3((unsigned)(tiles < fit ? tiles : fit), 1, 1), 32 * I8R_WARPS, int8_list_bytes(p.experts), s, dependent, p);
+}
+// Which form of the kernel takes a product; none where the tensor-core kernel of int8_pair.cu is the faster one. What decides is how many
+// 16-row tiles there are for 2368 warps, and how many tokens meet each weight. us, quantizer included, bf16, weights out of HBM (pair: the
+// tensor-core kernel):
+//   up to 8 tokens   8 warps a tile: 4096 x 1024 4.5 (4: 5.5, pair 10.8), 4096 x 4096 6.4 (4: 7.0), 14336 x 4096 13.5 (4: 16.5, pair 22.8)
+//                    4 warps:        one token through 2 of 8 experts of 4096 x 14336 68.9 (8: 72.7)
+//                    2 warps and 32 rows: 4096 x 28672 21.8 (4: 22.6, pair 24.3); 16 tokens through 8 of 128 experts of 2048 x 768 67.8
+//                    (4 warps, 16 rows: 78.2, pair 73.5). Experts with five tokens and more: pair (48 tokens through 6 of 64: 97.8, 98.5)
+//   more, 16 at once 16 rows:        16 tokens 4096 x 4096 7.2 (pair 11.1), 14336 x 4096 15.5 (pair 22.7); 64 tokens 4096 x 1024 6.4
+//                    32 rows:        32 tokens 4096 x 4096 8.8 (16 rows 9.7, pair 11.3), 14336 x 4096 21.4 (24.1, pair 23.2)
+//                    none:           16 tokens 4096 x 14336 16.5 (pair 15.2), 32 tokens 24.6 (15.5), 64 tokens 4096 x 4096 13.8 (11.5)
+enum class RowsForm { none, few_tiles, some_tiles, many_tiles, tokens16, tokens32 };
+static RowsForm rows_form(const Int8Product& p) {
+    const int used = p.experts < p.rows ? p.experts : p.rows;  // experts with tokens, at most
+    const int per = (p.rows + used - 1) / used;
+    const long long tiles = (long long)((p.n + 15) / 16) * used;
+    if (per <= 8 && tiles < 1536) return tiles < 512 ? RowsForm::few_tiles : RowsForm::some_tiles;
+    if (per <= (p.experts > 1 ? 4 : 8)) return RowsForm::many_tiles;
+    const long long groups = (per + 15) / 16 * tiles;
+    if (groups <= 512) return groups <= 256 || per <= 16 ? RowsForm::tokens16 : RowsForm::tokens32;
+    return RowsForm::none;
+}
+bool int8_rows_pays(const Int8Product& p) { return rows_form(p) != RowsForm::none; }
+
 template <typename OutT> static cudaError_t rows_t(const Int8Product& p, cudaStream_t s, bool dependent) {
-    const int per = p.experts > 1 ? (p.rows + p.experts - 1) / p.experts : p.rows;  // tokens of an expert, on average
-    const int r16 = (p.n + 15) / 16, r32 = (p.n + 31) / 32;
-    if (per <= 8) return launch_kernel(int8_rows_kernel<OutT, 1, 1>, dim3(r16, p.experts), 32 * I8R_WARPS, 0, s, dependent, p);
-    if (per <= 16) return launch_kernel(int8_rows_kernel<OutT, 1, 2>, dim3(r16, p.experts), 32 * I8R_WARPS, 0, s, dependent, p);
-    return launch_kernel(int8_rows_kernel<OutT, 2, 4>, dim3(r32, p.experts), 32 * I8R_WARPS, 0, s, dependent, p);
+    switch (rows_form(p)) {
+        case RowsForm::few_tiles: return rows_launch<OutT, 1, 1, 4, 8, 2>(p, s, dependent);
+        case RowsForm::some_tiles: return rows_launch<OutT, 1, 1, 4, 4, 2>(p, s, dependent);
+        case RowsForm::many_tiles: return rows_launch<OutT, 2, 1, 2, 2, 2>(p, s, dependent);
+        case RowsForm::tokens16: return rows_launch<OutT, 1, 2, 2, 8, 2>(p, s, dependent);
+        default: return rows_launch<OutT, 2, 2, 1, 8, 2>(p, s, dependent);
+    }
 }
 
 cudaError_t int8_product_rows(int elem, const Int8Product& p, cudaStream_t s, bool dependent) {

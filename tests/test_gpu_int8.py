@@ -133,9 +133,9 @@ def check_product(m, n, k, dtype, seed=0):
 
 
 @pytest.mark.parametrize("m", ROWS)
-@pytest.mark.parametrize("n,k", [(1, 1), (72, 100), (1000, 1040), (513, 4096)])
+@pytest.mark.parametrize("n,k", [(1, 1), (72, 100), (1000, 1040), (513, 4096), (9001, 70), (25000, 200)])
 def test_products(m, n, k):
-    for dtype in DTYPES:
+    for dtype in DTYPES if n < 9000 else DTYPES[m % 3:m % 3 + 1]:
         check_product(m, n, k, dtype)
     assert_device_ok()
 
