@@ -11,56 +11,64 @@
 
 namespace b200q {
 
-constexpr int RT_THREADS = 512;
+constexpr int RT_THREADS = 1024;
+constexpr int RT_HELD = 8;      // ids that a lane reads at once
+constexpr int RT_ROW_THREADS = 256;
 
 // One CTA per expert, and one more for the slots of none. Each CTA counts by itself how many slots belong to experts before its own
 // (its first row) and ranks its own slots, reading all ids twice: a few hundred KB out of L2 at most, where counting once and ranking
-// afterwards would take two launches or CTAs that wait for one another.
+// afterwards would take two launches or CTAs that wait for one another. Up to 8192 slots a warp's ids stay in registers in between.
 template <typename Id>
 __global__ void __launch_bounds__(RT_THREADS) route_sort_kernel(const Id* __restrict__ ids, int slots, int experts, int* __restrict__ order,
                                                                int* __restrict__ offsets, int* __restrict__ position) {
-    __shared__ int before[RT_THREADS / 32 + 1], lower[RT_THREADS / 32];
+    constexpr int WARPS = RT_THREADS / 32, CHUNK = 32 * RT_HELD;
+    __shared__ int before[WARPS], lower[WARPS];
     grid_launch_dependents();
     const int e = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int WARPS = RT_THREADS / 32;
-    // a warp ranks a contiguous piece of the slots, 32 at a time
-    const int piece = ((slots + WARPS - 1) / WARPS + 31) & ~31;
-    const int from = min(warp * piece, slots), to = min(from + piece, slots);
-    const auto expert_of = [&](int i) {
-        const long long id = i < to ? (long long)ids[i] : -1;
-        return id >= 0 && id < experts ? (int)id : experts;  // `experts`: of none
+    // a warp ranks a contiguous piece of the slots
+    const int piece = ((slots + WARPS - 1) / WARPS + CHUNK - 1) / CHUNK * CHUNK;
+    const int from = (int)min((long long)warp * piece, (long long)slots), to = min(from + piece, slots);
+    int held[RT_HELD];
+    const auto read = [&](int i) {
+        Id raw[RT_HELD];
+#pragma unroll
+        for (int j = 0; j < RT_HELD; ++j) raw[j] = i + 32 * j + lane < to ? ids[i + 32 * j + lane] : (Id)-1;
+#pragma unroll
+        for (int j = 0; j < RT_HELD; ++j) held[j] = raw[j] >= 0 && raw[j] < experts ? (int)raw[j] : (i + 32 * j + lane < to ? experts : -1);  // `experts`: of none
     };
     int mine = 0, less = 0;
-    for (int i = from; i < to; i += 32) {
-        const int id = expert_of(i + lane);
-        mine += __popc(__ballot_sync(0xffffffffu, i + lane < to && id == e));
-        less += __popc(__ballot_sync(0xffffffffu, i + lane < to && id < e));
+    for (int i = from; i < to; i += CHUNK) {
+        read(i);
+#pragma unroll
+        for (int j = 0; j < RT_HELD; ++j) {
+            mine += __popc(__ballot_sync(0xffffffffu, held[j] == e));
+            less += __popc(__ballot_sync(0xffffffffu, held[j] >= 0 && held[j] < e));
+        }
     }
     if (lane == 0) {
-        before[warp + 1] = mine;
+        before[warp] = mine;
         lower[warp] = less;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int sum = 0;
-        for (int w = 0; w < WARPS; ++w) sum += lower[w];
-        before[0] = sum;
-        offsets[e] = sum;  // of e = experts: how many rows there are
-        for (int w = 0; w < WARPS; ++w) before[w + 1] += before[w];
-    }
-    __syncthreads();
-    int row = before[warp];
-    for (int i = from; i < to; i += 32) {
-        const bool is = i + lane < to && expert_of(i + lane) == e;
-        const unsigned vote = __ballot_sync(0xffffffffu, is);
-        if (is) {
-            const int r = row + __popc(vote & ((1u << lane) - 1));
-            position[i + lane] = e < experts ? r : -1;
-            order[r] = e < experts ? i + lane : -1;
+    // this warp's first row: the slots of lower experts, and those of this one in earlier pieces
+    const int first = __reduce_add_sync(0xffffffffu, lower[lane]);
+    int row = first + __reduce_add_sync(0xffffffffu, lane < warp ? before[lane] : 0);
+    if (threadIdx.x == 0) offsets[e] = first;  // of e = experts: how many rows there are
+    for (int i = from; i < to; i += CHUNK) {
+        if (piece > CHUNK) read(i);
+#pragma unroll
+        for (int j = 0; j < RT_HELD; ++j) {
+            const unsigned vote = __ballot_sync(0xffffffffu, held[j] == e);
+            if (held[j] == e) {
+                const int r = row + __popc(vote & ((1u << lane) - 1)), slot = i + 32 * j + lane;
+                position[slot] = e < experts ? r : -1;
+                order[r] = e < experts ? slot : -1;
+            }
+            row += __popc(vote);
         }
-        row += __popc(vote);
     }
 }
+static_assert(RT_THREADS == 1024, "a lane per warp adds up the warps' counts");
 
 cudaError_t route_sort(const void* ids, bool wide, int slots, int experts, int* order, int* offsets, int* position, cudaStream_t s) {
     const dim3 grid((unsigned)experts + 1, 1, 1);
@@ -68,87 +76,119 @@ cudaError_t route_sort(const void* ids, bool wide, int slots, int experts, int* 
     return launch_kernel(route_sort_kernel<int>, grid, RT_THREADS, 0, s, false, static_cast<const int*>(ids), slots, experts, order, offsets, position);
 }
 
-// V neighbouring values of a row, V = 1 or 16 bytes' worth of the narrowest type involved
+// V neighbouring values of a row as they lie in memory: 1, or 4 or 8, as many as fill the 16 bytes of a store (two half-filled stores per
+// lane would leave every sector half written)
 template <typename T, int V> struct Values {
-    float v[V];
-    __device__ void load(const T* p) {
+    alignas(V == 1 ? sizeof(T) : (V * sizeof(T) >= 16 ? 16 : 8)) T raw[V];
+    __device__ __forceinline__ void load(const T* p) {
         if constexpr (V == 1) {
-            v[0] = to_float<T>(*p);
+            raw[0] = *p;
+        } else if constexpr (V * sizeof(T) == 8) {
+            *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
         } else {
-            alignas(16) T raw[V];
 #pragma unroll
             for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(raw)[i] = *(reinterpret_cast<const uint4*>(p) + i);
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = to_float<T>(raw[i]);
         }
     }
-    __device__ void store(T* p) const {
+    __device__ __forceinline__ void store(T* p) const {
         if constexpr (V == 1) {
-            *p = from_float<T>(v[0]);
-        } else {
-            alignas(16) T raw[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) raw[i] = from_float<T>(v[i]);
+            *p = raw[0];
+        } else {  // (never less than 16 bytes)
 #pragma unroll
             for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(raw)[i];
         }
     }
+    __device__ __forceinline__ float get(int i) const { return to_float<T>(raw[i]); }
+    __device__ __forceinline__ void set(int i, float v) { raw[i] = from_float<T>(v); }
 };
 static bool rows_wide(const void* p, long long ld, int elem) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (elem == ELEM_F32 ? 4 : 2) % 16 == 0;
 }
 
+// The rows of slots j.. of a token: -1 where there is none.
+template <int S> __device__ __forceinline__ void slot_rows(const int* position, long long token, int topk, int j, int limit, int (&p)[S]) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) p[i] = j + i < topk ? position[token * topk + j + i] : -1;
+#pragma unroll
+    for (int i = 0; i < S; ++i) p[i] = p[i] < limit ? p[i] : -1;
+}
+
 // A CTA per token reads it once and writes its rows; rows behind the last are zeroed by the CTA that they would have belonged to had no
 // slot been left out.
-template <typename U>
-__global__ void __launch_bounds__(256) route_dispatch_kernel(const U* __restrict__ x, long long ldx, const int* __restrict__ position,
+template <typename U, int S>
+__global__ void __launch_bounds__(RT_ROW_THREADS) route_dispatch_kernel(const U* __restrict__ x, long long ldx, const int* __restrict__ position,
                                                              const int* __restrict__ valid, U* __restrict__ rows, int topk, int h) {
-    const int t = blockIdx.x;
-    const U* src = x + (long long)t * ldx;
+    const long long t = blockIdx.x;
+    const U* src = x + t * ldx;
     const int nvalid = min(*valid, (int)gridDim.x * topk);
     U zero{};
-    for (int c = threadIdx.x; c < h; c += 256) {
-        const U v = src[c];
-        for (int j = 0; j < topk; ++j) {
-            const long long r = (long long)t * topk + j;
-            const int p = position[r];
-            if (p >= 0 && p < nvalid) rows[(long long)p * h + c] = v;
-            if (r >= nvalid) rows[r * h + c] = zero;
+    for (int j = 0; j < topk; j += S) {
+        int p[S];
+        slot_rows(position, t, topk, j, nvalid, p);
+        for (int c = threadIdx.x; c < h; c += blockDim.x) {
+            const U v = src[c];
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                if (p[i] >= 0) rows[(long long)p[i] * h + c] = v;
+                if (j + i < topk && t * topk + j + i >= nvalid) rows[(t * topk + j + i) * h + c] = zero;
+            }
         }
     }
 }
+
+// threads of a CTA that goes over `n` pieces of a row
+static unsigned row_threads(int n) { return n >= RT_ROW_THREADS ? (unsigned)RT_ROW_THREADS : (unsigned)((n + 31) / 32 * 32); }
 
 cudaError_t route_dispatch(int elem, const void* x, long long ldx, const int* position, const int* valid, void* rows, int tokens, int topk, int h,
                            cudaStream_t s) {
     const int es = elem == ELEM_F32 ? 4 : 2;
     const dim3 grid((unsigned)tokens, 1, 1);
-    if (rows_wide(x, ldx, elem) && rows_wide(rows, h, elem))
-        return launch_kernel(route_dispatch_kernel<uint4>, grid, 256, 0, s, false, static_cast<const uint4*>(x), ldx * es / 16, position, valid, static_cast<uint4*>(rows), topk, h * es / 16);
-    if (es == 4) return launch_kernel(route_dispatch_kernel<uint32_t>, grid, 256, 0, s, false, static_cast<const uint32_t*>(x), ldx, position, valid, static_cast<uint32_t*>(rows), topk, h);
-    return launch_kernel(route_dispatch_kernel<uint16_t>, grid, 256, 0, s, false, static_cast<const uint16_t*>(x), ldx, position, valid, static_cast<uint16_t*>(rows), topk, h);
+    const auto go = [&](auto unit, int per) {  // `per` values in a unit
+        using U = decltype(unit);
+        const auto kernel = topk <= 2 ? route_dispatch_kernel<U, 2> : route_dispatch_kernel<U, 4>;
+        return launch_kernel(kernel, grid, row_threads(h / per), 0, s, false, static_cast<const U*>(x), ldx / per, position, valid, static_cast<U*>(rows), topk, h / per);
+    };
+    if (rows_wide(x, ldx, elem) && rows_wide(rows, h, elem)) return go(uint4{}, 16 / es);
+    if (es == 4) return go(uint32_t{}, 1);
+    return go(uint16_t{}, 1);
 }
 
-// out[t] = sum_j weights[t, j] rows[position[t, j]]; weights null: 1.
-template <typename In, typename Out, int V>
-__global__ void __launch_bounds__(256) route_combine_kernel(const In* rows, long long ldr, const int* position, const float* weights, Out* out, int topk,
+// out[t] = sum_j weights[t, j] rows[position[t, j]]; weights null: 1. The loads of four slots' rows are under way at once: one after the
+// other, eight slots of seven tokens took 7.4 us.
+template <typename In, typename Out, int V, int S>
+__global__ void __launch_bounds__(RT_ROW_THREADS) route_combine_kernel(const In* rows, long long ldr, const int* position, const float* weights, Out* out, int topk,
                                                             int h) {
     grid_dependency_wait();
     grid_launch_dependents();
     const long long t = blockIdx.x;
-    for (int c = V * threadIdx.x; c < h; c += V * 256) {
-        Values<Out, V> sum;
+    const int limit = (int)gridDim.x * topk;
+    int p[S];
+    float w[S];
+    const auto slots = [&](int j) {
+        slot_rows(position, t, topk, j, limit, p);
 #pragma unroll
-        for (int i = 0; i < V; ++i) sum.v[i] = 0.0f;
-        for (int j = 0; j < topk; ++j) {
-            const int p = position[t * topk + j];
-            if (p < 0 || p >= (int)gridDim.x * topk) continue;
-            const float w = weights != nullptr ? weights[t * topk + j] : 1.0f;
-            Values<In, V> r;
-            r.load(rows + p * ldr + c);
+        for (int i = 0; i < S; ++i) w[i] = weights == nullptr ? 1.0f : (j + i < topk ? weights[t * topk + j + i] : 0.0f);
+    };
+    slots(0);
+    for (int c = V * threadIdx.x; c < h; c += V * blockDim.x) {
+        float sum[V] = {};
+        for (int j = 0; j < topk; j += S) {
+            if (topk > S) slots(j);
+            Values<In, V> r[S];
 #pragma unroll
-            for (int i = 0; i < V; ++i) sum.v[i] = fmaf(w, r.v[i], sum.v[i]);
+            for (int i = 0; i < S; ++i)
+                if (p[i] >= 0) r[i].load(rows + p[i] * ldr + c);
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+                if (p[i] >= 0) {
+#pragma unroll
+                    for (int k = 0; k < V; ++k) sum[k] = fmaf(w[i], r[i].get(k), sum[k]);
+                }
         }
-        sum.store(out + t * h + c);
+        Values<Out, V> v;
+#pragma unroll
+        for (int k = 0; k < V; ++k) v.set(k, sum[k]);
+        v.store(out + t * h + c);
     }
 }
 
@@ -156,8 +196,9 @@ template <typename In, typename Out>
 static cudaError_t combine_t(bool wide, const void* rows, long long ldr, const int* position, const float* weights, void* out, int tokens, int topk,
                              int h, cudaStream_t s, bool dependent) {
     const dim3 grid((unsigned)tokens, 1, 1);
-    if (wide) return launch_kernel(route_combine_kernel<In, Out, 8>, grid, 256, 0, s, dependent, static_cast<const In*>(rows), ldr, position, weights, static_cast<Out*>(out), topk, h);
-    return launch_kernel(route_combine_kernel<In, Out, 1>, grid, 256, 0, s, dependent, static_cast<const In*>(rows), ldr, position, weights, static_cast<Out*>(out), topk, h);
+    constexpr int V = 16 / sizeof(Out);
+    const auto kernel = wide ? (topk <= 2 ? route_combine_kernel<In, Out, V, 2> : route_combine_kernel<In, Out, V, 4>) : route_combine_kernel<In, Out, 1, 4>;
+    return launch_kernel(kernel, grid, row_threads(wide ? h / V : h), 0, s, dependent, static_cast<const In*>(rows), ldr, position, weights, static_cast<Out*>(out), topk, h);
 }
 cudaError_t route_combine(int elem_in, int elem_out, const void* rows, long long ldr, const int* position, const float* weights, void* out,
                           int tokens, int topk, int h, cudaStream_t s, bool dependent) {
@@ -177,53 +218,65 @@ cudaError_t route_combine(int elem_in, int elem_out, const void* rows, long long
     return combine_t<__nv_bfloat16, __nv_bfloat16>(wide, rows, ldr, position, weights, out, tokens, topk, h, s, dependent);
 }
 
-// The gradients of combine, a CTA per token: its slots' rows of drows (each written by one CTA), and the products with the rows. Rows
-// behind the last become zeros as in dispatch. Either output may be left out (null).
-template <typename G, typename T, int V>
-__global__ void __launch_bounds__(256) route_combine_grad_kernel(const G* __restrict__ grad_out, long long ldg, const T* __restrict__ rows, long long ldr,
+// The gradients of combine, a CTA per token: its slots' rows of drows (each written by one CTA), and the products with the rows, four
+// slots at a time. Rows behind the last become zeros as in dispatch. Either output may be left out (null).
+template <typename G, typename T, int V, int S>
+__global__ void __launch_bounds__(RT_ROW_THREADS) route_combine_grad_kernel(const G* __restrict__ grad_out, long long ldg, const T* __restrict__ rows, long long ldr,
                                                                  const int* __restrict__ position, const int* __restrict__ valid,
                                                                  const float* __restrict__ weights, T* __restrict__ grad_rows,
                                                                  float* __restrict__ grad_weights, int topk, int h) {
-    __shared__ float part[8];
+    __shared__ float part[S][RT_ROW_THREADS / 32];
     const long long t = blockIdx.x;
     const int nvalid = min(*valid, (int)gridDim.x * topk), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int j = 0; j < topk; ++j) {
-        const long long slot = t * topk + j;
-        const int p = position[slot];
-        float dot = 0.0f;
-        if (p >= 0 && p < nvalid) {
-            const float w = weights[slot];
-            for (int c = V * threadIdx.x; c < h; c += V * 256) {
-                Values<G, V> g;
-                g.load(grad_out + t * ldg + c);
-                if (grad_weights != nullptr) {
-                    Values<T, V> r;
-                    r.load(rows + p * ldr + c);
+    for (int j = 0; j < topk; j += S) {
+        int p[S];
+        slot_rows(position, t, topk, j, nvalid, p);
+        float w[S], dot[S] = {};
 #pragma unroll
-                    for (int i = 0; i < V; ++i) dot = fmaf(g.v[i], r.v[i], dot);
-                }
-                if (grad_rows != nullptr) {
+        for (int i = 0; i < S; ++i) w[i] = j + i < topk ? weights[t * topk + j + i] : 0.0f;
+        for (int c = V * threadIdx.x; c < h; c += V * blockDim.x) {
+            Values<G, V> g;
+            g.load(grad_out + t * ldg + c);
+            if (grad_weights != nullptr) {
+                Values<T, V> r[S];
+#pragma unroll
+                for (int i = 0; i < S; ++i)
+                    if (p[i] >= 0) r[i].load(rows + p[i] * ldr + c);
+#pragma unroll
+                for (int i = 0; i < S; ++i)
+                    if (p[i] >= 0) {
+#pragma unroll
+                        for (int k = 0; k < V; ++k) dot[i] = fmaf(g.get(k), r[i].get(k), dot[i]);
+                    }
+            }
+            if (grad_rows != nullptr) {
+#pragma unroll
+                for (int i = 0; i < S; ++i) {
                     Values<T, V> d;
+                    if (p[i] >= 0) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) d.v[i] = w * g.v[i];
-                    d.store(grad_rows + (long long)p * h + c);
+                        for (int k = 0; k < V; ++k) d.set(k, w[i] * g.get(k));
+                        d.store(grad_rows + (long long)p[i] * h + c);
+                    }
+                    if (j + i < topk && t * topk + j + i >= nvalid) {
+#pragma unroll
+                        for (int k = 0; k < V; ++k) d.set(k, 0.0f);
+                        d.store(grad_rows + (t * topk + j + i) * h + c);
+                    }
                 }
             }
         }
-        if (grad_rows != nullptr && slot >= nvalid) {
-            Values<T, V> zero;
-#pragma unroll
-            for (int i = 0; i < V; ++i) zero.v[i] = 0.0f;
-            for (int c = V * threadIdx.x; c < h; c += V * 256) zero.store(grad_rows + slot * h + c);
-        }
         if (grad_weights != nullptr) {
-            dot = warp_sum(dot);
-            if (lane == 0) part[warp] = dot;
+#pragma unroll
+            for (int i = 0; i < S; ++i) {
+                const float sum = warp_sum(dot[i]);
+                if (lane == 0) part[i][warp] = sum;
+            }
             __syncthreads();
-            if (threadIdx.x == 0) {
+            if (threadIdx.x < S && j + (int)threadIdx.x < topk) {
                 float sum = 0.0f;
-                for (int i = 0; i < 8; ++i) sum += part[i];
-                grad_weights[slot] = sum;
+                for (int i = 0; i < (int)(blockDim.x >> 5); ++i) sum += part[threadIdx.x][i];
+                grad_weights[t * topk + j + threadIdx.x] = sum;
             }
             __syncthreads();
         }
@@ -237,8 +290,9 @@ static cudaError_t combine_grad_t(bool wide, const void* grad_out, long long ldg
     const G* g = static_cast<const G*>(grad_out);
     const T* r = static_cast<const T*>(rows);
     T* d = static_cast<T*>(grad_rows);
-    if (wide) return launch_kernel(route_combine_grad_kernel<G, T, 8>, grid, 256, 0, s, false, g, ldg, r, ldr, position, valid, weights, d, grad_weights, topk, h);
-    return launch_kernel(route_combine_grad_kernel<G, T, 1>, grid, 256, 0, s, false, g, ldg, r, ldr, position, valid, weights, d, grad_weights, topk, h);
+    constexpr int V = 16 / sizeof(T);
+    const auto kernel = wide ? (topk <= 2 ? route_combine_grad_kernel<G, T, V, 2> : route_combine_grad_kernel<G, T, V, 4>) : route_combine_grad_kernel<G, T, 1, 4>;
+    return launch_kernel(kernel, grid, h >= 8 ? row_threads(wide ? h / V : h) : 32u, 0, s, false, g, ldg, r, ldr, position, valid, weights, d, grad_weights, topk, h);
 }
 cudaError_t route_combine_grad(int elem_grad, int elem, const void* grad_out, long long ldg, const void* rows, long long ldr, const int* position,
                                const int* valid, const float* weights, void* grad_rows, float* grad_weights, int tokens, int topk, int h,

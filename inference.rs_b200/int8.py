@@ -42,7 +42,9 @@ class Int8Tensor:
     @classmethod
     def _of_rows(cls, q: torch.Tensor, scales: torch.Tensor, shape: tuple[int, ...]) -> "Int8Tensor":
         self = cls.__new__(cls)
-        self.shape, self.data, self.scales = shape, q.view(*shape[:-1], q.shape[-1]), scales.view(shape[:-1])
+        self.shape, self.data, self.scales = shape, q, scales
+        if len(shape) == 3:
+            self.data, self.scales = q.view(*shape[:-1], q.shape[-1]), scales.view(shape[:-1])
         return self
 
     @classmethod
@@ -50,7 +52,7 @@ class Int8Tensor:
         """A weight [n, k] or [experts, n, k] of f32, f16 or bf16, each row with the scale max|row| / 127."""
         if src.dim() not in (2, 3):
             raise ValueError(f"quantize takes a matrix, or one per expert, got {tuple(src.shape)}")
-        return cls._of_rows(*ops.int8_quantize(src.detach().reshape(-1, src.shape[-1])), tuple(src.shape))
+        return cls._of_rows(*ops.int8_quantize(src if src.dim() == 2 else src.detach().reshape(-1, src.shape[-1])), tuple(src.shape))
 
     @classmethod
     def from_qtensor(cls, *weights: QTensor) -> "Int8Tensor":
