@@ -4,7 +4,7 @@ for a random-initialised model in the Q4_K_M mix, and a loader that hands the pr
 The reference maps GGUF tensor names to its layers' checkpoint-style names when it loads a llama-family file
 (crates/inference-gguf/src/normal_bindings.rs:887-914: `blk.N.attn_q` -> `model.layers.N.self_attn.q_proj`, ...; the
 non-layer tensors `token_embd`, `output_norm`, `output` in the same function). Only what the matmul path needs is here:
-the seven projections per layer, the output head and the embedding table.
+the seven projections per layer, the output head and the embedding table, and the stacked matrices of a layer of experts.
 """
 from __future__ import annotations
 
@@ -127,3 +127,34 @@ def load_projections(f: BinaryIO, content: Content, device="cuda"):
                 raise GgufError(f"{name}: shape {tuple(info.shape)}, the metadata implies {(n, k)}")
         out[target] = content.tensor(f, name, device)
     return out
+
+
+# the stacked matrices of a layer of experts, [experts, n, k] each (llama.cpp's names)
+EXPERT_TENSORS = ("ffn_gate_exps", "ffn_up_exps", "ffn_down_exps")
+
+
+def load_experts(f: BinaryIO, content: Content, layer: int, activation: str = "silu", device="cuda"):
+    """`Int8Experts` of layer `layer` from its stacked Q8_0 / Q4_K / Q6_K matrices: each expert's blocks are brought over, expanded and
+    quantized again with a scale per row on the device, one expert at a time."""
+    import torch
+
+    from .int8 import Int8Experts, Int8Tensor
+    from .qmatmul import QTensor
+    parts, shapes = [], []
+    for key in EXPERT_TENSORS:
+        name = f"blk.{layer}.{key}.weight"
+        info, raw = content.tensor_bytes(f, name)
+        if info.ggml_dtype not in (int(GgmlDType.Q8_0), int(GgmlDType.Q4K), int(GgmlDType.Q6K)):
+            raise GgufError(f"{name}: ggml type {info.ggml_dtype} is not one of Q8_0, Q4_K, Q6_K")
+        if len(info.shape) != 3:
+            raise GgufError(f"{name}: shape {tuple(info.shape)}, expected one matrix per expert")
+        parts.append((GgmlDType(info.ggml_dtype), raw))
+        shapes.append(tuple(info.shape))
+    experts, ffn, hidden = shapes[0]
+    if shapes != [(experts, ffn, hidden), (experts, ffn, hidden), (experts, hidden, ffn)]:
+        raise GgufError(f"blk.{layer}: gate {shapes[0]}, up {shapes[1]}, down {shapes[2]} do not make a layer of experts")
+    tensors = []
+    for (dtype, raw), (_, n, k) in zip(parts, shapes):
+        each = [Int8Tensor.from_qtensor(QTensor.from_packed(one, dtype, (n, k), device)) for one in raw.reshape(experts, -1)]
+        tensors.append(Int8Tensor(torch.stack([t.data[:, :k] for t in each]), torch.stack([t.scales for t in each])))
+    return Int8Experts(*tensors, activation=activation)

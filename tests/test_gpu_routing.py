@@ -205,6 +205,45 @@ def test_in_graphs_and_on_other_streams():
         assert all(torch.equal(a, b) for a, b in zip(again, want))
 
 
+def test_a_captured_backward_pass():
+    ids, w = choose(40, 6, 3, 0.2), torch.rand(40, 3, device="cuda")
+    x, go, gr = values(40, 72, torch.bfloat16, 1), values(40, 72, torch.bfloat16, 2), values(120, 72, torch.bfloat16, 3)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, w)]
+        r = pkg.TokenRouting(ids, 6)
+        rows = r.dispatch(leaves[0])
+        return torch.autograd.grad([rows, r.combine(rows, leaves[1])], leaves, [gr, go])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        grads = step()
+    for seed in (4, 5):
+        ids.copy_(choose(40, 6, 3, 0.3, seed=seed))
+        x.copy_(values(40, 72, torch.bfloat16, seed))
+        w.copy_(torch.rand(40, 3, device="cuda"))
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(grads, step()))
+
+
+def test_no_tokens_and_narrow_rows():
+    r = pkg.TokenRouting(torch.zeros(0, 3, dtype=torch.int32, device="cuda"), 4)
+    assert r.dispatch(torch.zeros(0, 8, device="cuda")).shape == (0, 8) and r.offsets.tolist() == [0] * 5
+    assert r.combine(torch.zeros(0, 8, device="cuda"), torch.zeros(0, 3, device="cuda")).shape == (0, 8)
+    r = pkg.TokenRouting(choose(5, 4, 2, 0.0), 4)
+    x, w = torch.zeros(5, 0, device="cuda", requires_grad=True), torch.ones(5, 2, device="cuda", requires_grad=True)
+    rows = r.dispatch(x)
+    out = r.combine(rows, w)
+    assert rows.shape == (10, 0) and out.shape == (5, 0)
+    gx, gw = torch.autograd.grad([out], [x, w], [torch.zeros(5, 0, device="cuda")])
+    assert gx.shape == (5, 0) and not gw.any()
+
+
 def test_beyond_32_bit_offsets():
     tokens, topk, h = 300000, 2, 4096  # 2.46e9 values in the rows
     ids = torch.randint(0, 7, (tokens, topk), device="cuda")
