@@ -66,8 +66,8 @@ __device__ __noinline__ uint32_t quantize_four_carefully(float a, float b, float
 // times one 8-bit mantissa by another), so a way out of line for them was taken by every other warp and cost as much as all the rest.
 // HALVES: a value can lie on a half exactly without s being a power of two, for which the rounding of x * (1 / s) is right as it is. Not
 // so for bf16: half an odd multiple of s has 8 bits only where s has one.
+// Rows of the smallest floats (r.pre) are not for this one.
 template <bool HALVES> __device__ __forceinline__ uint32_t quantize_four(float a, float b, float c, float d, const RowScale& r) {
-    if (r.pre != 1.0f) return quantize_four_carefully(a, b, c, d, r.sn, r.inv, r.pre);
     const float v[4] = {a, b, c, d};
     float t[4];
     bool on_half = false;
@@ -76,15 +76,21 @@ template <bool HALVES> __device__ __forceinline__ uint32_t quantize_four(float a
         t[i] = fmaf(v[i], r.inv, ROUND);
         const float rem = fmaf(ROUND - t[i], r.sn, v[i]);
         if constexpr (HALVES) on_half |= fabsf(rem) == r.half;
-        if (fabsf(rem) > r.half) t[i] += copysignf(1.0f, rem);
+        const float step = __uint_as_float((__float_as_uint(rem) & 0x80000000u) | 0x3f800000u);
+        t[i] = fabsf(rem) > r.half ? t[i] + step : t[i];
     }
     if (HALVES && on_half) return quantize_four_carefully(a, b, c, d, r.sn, r.inv, 1.0f);
     return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
 }
 
+template <bool HALVES> __device__ __forceinline__ uint32_t quantize_any(float a, float b, float c, float d, const RowScale& r) {
+    if (r.inv == 0.0f) return 0u;
+    return r.pre == 1.0f ? quantize_four<HALVES>(a, b, c, d, r) : quantize_four_carefully(a, b, c, d, r.sn, r.inv, r.pre);
+}
+
 // Eight values of a row as they lie in memory. Plain loads: what they read may be the work of the launch before, which this one waited
-// for after it had started. `top` is the largest magnitude as a bit pattern of the type: patterns without their sign are in the order of
-// the values, with infinities and NaN above all.
+// for after it had started. `top` is the largest magnitude, `float_bits` its pattern as a float: patterns without their sign are in the
+// order of the values, with infinities and NaN above all.
 template <typename T> struct Eight;
 template <> struct Eight<float> {
     float4 a, b;
@@ -99,25 +105,41 @@ template <> struct Eight<float> {
         return max(m, max(max(abs_bits(b.x), abs_bits(b.y)), max(abs_bits(b.z), abs_bits(b.w))));
     }
     static __device__ uint32_t float_bits(uint32_t top) { return top; }
-    __device__ uint2 quantize(const RowScale& r) const { return make_uint2(quantize_four<true>(a.x, a.y, a.z, a.w, r), quantize_four<true>(b.x, b.y, b.z, b.w, r)); }
+    static constexpr bool HALVES = true;
+    __device__ void get(float (&v)[8]) const {
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
 };
 template <typename T> struct Eight {
     uint4 a;
     __device__ void load(const T* p) { a = *reinterpret_cast<const uint4*>(p); }
     __device__ void zero() { a = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ uint32_t top(uint32_t m) const {  // two patterns side by side
-        const uint32_t lo = __vmaxu2(a.x & 0x7fff7fffu, a.y & 0x7fff7fffu), hi = __vmaxu2(a.z & 0x7fff7fffu, a.w & 0x7fff7fffu);
-        return __vmaxu2(m, __vmaxu2(lo, hi));
+    using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    __device__ uint32_t top(uint32_t m) const {  // two values side by side, a NaN above all
+        const Pair* w = reinterpret_cast<const Pair*>(&a);
+        const Pair lo = __hmax2_nan(__habs2(w[0]), __habs2(w[1])), hi = __hmax2_nan(__habs2(w[2]), __habs2(w[3]));
+        const Pair r = __hmax2_nan(*reinterpret_cast<const Pair*>(&m), __hmax2_nan(lo, hi));
+        return *reinterpret_cast<const uint32_t*>(&r);
     }
     static __device__ uint32_t float_bits(uint32_t top) {
-        const unsigned short t = (unsigned short)max(top & 0xffffu, top >> 16);
-        return __float_as_uint(to_float<T>(*reinterpret_cast<const T*>(&t)));
+        const unsigned short lo = (unsigned short)top, hi = (unsigned short)(top >> 16);
+        return max(__float_as_uint(to_float<T>(*reinterpret_cast<const T*>(&lo))) & 0x7fffffffu, __float_as_uint(to_float<T>(*reinterpret_cast<const T*>(&hi))) & 0x7fffffffu);
     }
     static constexpr bool HALVES = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value;
-    __device__ uint2 quantize(const RowScale& r) const {
-        const T* e = reinterpret_cast<const T*>(&a);
-        return make_uint2(quantize_four<HALVES>(to_float<T>(e[0]), to_float<T>(e[1]), to_float<T>(e[2]), to_float<T>(e[3]), r),
-                          quantize_four<HALVES>(to_float<T>(e[4]), to_float<T>(e[5]), to_float<T>(e[6]), to_float<T>(e[7]), r));
+    __device__ void get(float (&v)[8]) const {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        } else {
+            const T* e = reinterpret_cast<const T*>(&a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = to_float<T>(e[i]);
+        }
     }
 };
 
@@ -166,7 +188,9 @@ template <typename T, int STEPS> struct RowPart {
         for (int i = 0; i < STEPS; ++i) {
             const int c = 8 * (rank + i * size);
             if (c >= kp) break;
-            const uint2 w = r.inv != 0.0f ? held[i].quantize(r) : make_uint2(0u, 0u);
+            float v[8];
+            held[i].get(v);
+            const uint2 w = make_uint2(quantize_any<Eight<T>::HALVES>(v[0], v[1], v[2], v[3], r), quantize_any<Eight<T>::HALVES>(v[4], v[5], v[6], v[7], r));
             if (p.position == nullptr) {
                 *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = w;
             } else {
@@ -220,7 +244,7 @@ template <typename T> __global__ void __launch_bounds__(256) int8_quantize_plain
         float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = c + j < p.k ? to_float<T>(x[c + j]) : 0.0f;
-        const uint32_t w = r.inv != 0.0f ? quantize_four<true>(v[0], v[1], v[2], v[3], r) : 0u;
+        const uint32_t w = quantize_any<true>(v[0], v[1], v[2], v[3], r);
         if (p.position == nullptr) {
             *reinterpret_cast<uint32_t*>(p.q + row * p.ldq + c) = w;
         } else {
