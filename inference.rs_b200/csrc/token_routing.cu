@@ -41,10 +41,12 @@ __global__ void __launch_bounds__(RT_THREADS) route_sort_kernel(const Id* __rest
         read(i);
 #pragma unroll
         for (int j = 0; j < RT_HELD; ++j) {
-            mine += __popc(__ballot_sync(0xffffffffu, held[j] == e));
-            less += __popc(__ballot_sync(0xffffffffu, held[j] >= 0 && held[j] < e));
+            mine += held[j] == e;
+            less += (unsigned)held[j] < (unsigned)e;  // (-1 is above)
         }
     }
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    less = __reduce_add_sync(0xffffffffu, less);
     if (lane == 0) {
         before[warp] = mine;
         lower[warp] = less;

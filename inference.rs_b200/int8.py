@@ -49,9 +49,12 @@ class Int8Tensor:
 
     @classmethod
     def quantize(cls, src: torch.Tensor) -> "Int8Tensor":
-        """A weight [n, k] or [experts, n, k] of f32, f16 or bf16, each row with the scale max|row| / 127."""
+        """A weight [n, k] or [experts, n, k] of f32, f16 or bf16, each row with the scale max|row| / 127; brought to the GPU where it is
+        not there."""
         if src.dim() not in (2, 3):
             raise ValueError(f"quantize takes a matrix, or one per expert, got {tuple(src.shape)}")
+        if not src.is_cuda:
+            src = src.cuda()
         return cls._of_rows(*ops.int8_quantize(src if src.dim() == 2 else src.detach().reshape(-1, src.shape[-1])), tuple(src.shape))
 
     @classmethod

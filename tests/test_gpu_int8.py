@@ -103,6 +103,12 @@ def test_a_value_that_is_not_finite_spoils_its_row_alone(dtype, value):
     assert y.isnan().all(1).tolist() == [False, False, True, False] and y[[0, 1, 3]].isfinite().all()
 
 
+def test_quantize_brings_host_weights_over():
+    w = torch.randn(3, 5, 24)
+    t = pkg.Int8Tensor.quantize(w)
+    assert t.shape == (3, 5, 24) and t.data.is_cuda and torch.equal(t.data, pkg.Int8Tensor.quantize(w.cuda()).data)
+
+
 def test_from_qtensor():
     g = torch.Generator(device="cuda").manual_seed(3)
     qs = [pkg.QTensor.quantize(torch.randn(48, 512, device="cuda", generator=g) * 0.02, t) for t in (pkg.GgmlDType.Q8_0, pkg.GgmlDType.Q4K)]
@@ -242,6 +248,40 @@ def test_rows_meet_their_experts_matrix(counts, n, k):
             want = (xq[at:at + c, :k].double() @ w.data[i, :, :k].double().T) * xs[at:at + c].double()[:, None] * w.scales[i].double()
             close(got[at:at + c], want)
             at += c
+    assert_device_ok()
+
+
+def check_experts(counts, n, k, dtype):
+    w, x = int8_weight(len(counts), n, k), acts(sum(counts), k, torch.float32)
+    xq, xs = ops.int8_quantize(x)
+    offsets = torch.tensor([0, *torch.tensor(counts).cumsum(0).tolist()], dtype=torch.int32, device="cuda")
+    got = ops.int8_gemm(xq, xs, w.data, w.scales, k, dtype, offsets)
+    at = 0
+    for i, c in enumerate(counts):
+        want = (xq[at:at + c, :k].double() @ w.data[i, :, :k].double().T) * xs[at:at + c].double()[:, None] * w.scales[i].double()
+        close(got[at:at + c], want)
+        at += c
+    assert_device_ok()
+
+
+def test_tiles_of_every_height():
+    check_experts([252, 31, 220, 60, 190, 90, 157, 125, 256, 513, 255, 1], 300, 272, torch.float32)
+
+
+def test_a_thousand_experts():
+    g = torch.Generator().manual_seed(2)
+    check_experts(torch.randint(0, 40, (1024,), generator=g).tolist(), 272, 100, torch.bfloat16)
+    check_experts((torch.rand(1024, generator=g) < 0.2).int().tolist(), 272, 100, torch.bfloat16)
+
+
+def test_offsets_that_lead_nowhere_are_harmless():
+    """Rows are taken from inside the buffers only, whatever the offsets say."""
+    w, x = int8_weight(4, 40, 64), acts(30, 64, torch.float32)
+    xq, xs = ops.int8_quantize(x)
+    for bad in ([5, 3, 90, -7, 2], [0, 10, 4, 2 ** 31 - 1, 2 ** 31 - 1], [-(2 ** 31)] * 5):
+        out = torch.full((32, 40), 7.0, device="cuda")
+        ops.int8_gemm(xq, xs, w.data, w.scales, 64, torch.float32, torch.tensor(bad, dtype=torch.int32, device="cuda"), out[:30])
+        assert (out[30:] == 7).all()
     assert_device_ok()
 
 
