@@ -9,23 +9,11 @@
 //
 // Every wait is bounded; a wait that gives up records a code in the device status word, work is skipped, and the kernel still frees its
 // TMEM columns before it returns.
-#include <cuda.h>
-
-#include "int8.cuh"
-#include "tcgen05.cuh"
+#include "int8_pair.cuh"
 
 namespace b200q {
 
-constexpr int I8P_ROWS = 128;      // weight rows of one CTA = TMEM lanes
-constexpr int I8P_TOKENS = 256;    // tokens of a tile at most = TMEM columns of one accumulator
-constexpr int I8P_BK = 128;        // k per stage: one 128-byte swizzled row
-constexpr int I8P_SUB = 2;         // such pieces per stage: the hand-over of a stage from TMA to tensor core and back takes as long as a
-                                   // small tile's products of 128 k (16 tokens, 16384 k: 345 cycles per 128 k with one, 275 with two)
-constexpr int I8P_MAX_STAGES = 6;
-constexpr int I8P_A_BYTES = I8P_ROWS * I8P_BK;
-constexpr int I8P_THREADS = 384;   // warp 0 TMA, warp 1 MMA, warp 2 TMEM, warps 4-11 epilogue
-constexpr int I8P_EPILOGUE = 8;    // warps: two to a quarter of the TMEM lanes, taking its columns 32 at a time in turn
-constexpr int I8P_TMEM_COLS = 512;
+constexpr int I8P_TMEM_COLS = 512;  // two accumulators
 
 struct Int8PairParams {
     Int8Product p;
@@ -41,8 +29,6 @@ struct Int8PairBarriers {
 static size_t i8p_smem(int stages, int bn, int experts) {
     return 1024 + (size_t)stages * I8P_SUB * (I8P_A_BYTES + bn / 2 * I8P_BK) + sizeof(Int8PairBarriers) + int8_list_bytes(experts);
 }
-
-__device__ __forceinline__ int tile_columns(int toks) { return (toks + 31) & ~31; }  // N of the instruction
 
 template <typename OutT, int ACT>  // ACT: INT8_ACT_NONE, or the activation of a gated product
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
@@ -279,22 +265,8 @@ template <typename OutT, int ACT> static int pair_t(const Int8Product& p, cudaSt
     pp.bn = int8_token_tile(p, pp.tiles_n);
     pp.stages = I8P_MAX_STAGES;
     while (i8p_smem(pp.stages, pp.bn, p.experts) > (size_t)runtime_info().smem_optin - 1024) --pp.stages;
-    const cuuint64_t kp = (cuuint64_t)((p.k + 15) & ~15);
     CUtensorMap map_w, map_x;
-    {
-        const cuuint64_t dims[2] = {kp, (cuuint64_t)p.experts * p.n};
-        const cuuint32_t box[2] = {I8P_BK, I8P_ROWS};
-        if (encode_tiled_2d_cached(&map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.wq, dims, (cuuint64_t)p.ldw, box, CU_TENSOR_MAP_SWIZZLE_128B,
-                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != CUDA_SUCCESS)
-            return set_error(B200Q_ERR_INVALID, "no tensor map for the weights");
-    }
-    {
-        const cuuint64_t dims[2] = {kp, (cuuint64_t)p.rows};
-        const cuuint32_t box[2] = {I8P_BK, (cuuint32_t)(pp.bn / 2)};
-        if (encode_tiled_2d_cached(&map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.xq, dims, (cuuint64_t)p.ldx, box, CU_TENSOR_MAP_SWIZZLE_128B,
-                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B) != CUDA_SUCCESS)
-            return set_error(B200Q_ERR_INVALID, "no tensor map for the activations");
-    }
+    if (!int8_pair_maps(p, pp.bn, &map_w, &map_x)) return set_error(B200Q_ERR_INVALID, "no tensor map for these rows");
     constexpr auto kernel = int8_pair_kernel<OutT, ACT>;
     cudaError_t e = allow_full_smem<kernel>();
     if (e == cudaSuccess) {
@@ -320,6 +292,8 @@ template <typename OutT> static int pair_out(const Int8Product& p, cudaStream_t 
 bool int8_pair_ready() { return encode_tiled_fn() != nullptr; }
 
 int int8_product_pair(int elem, const Int8Product& p, cudaStream_t s, bool dependent) {
+    const int rc = int8_product_split(elem, p, s, dependent);
+    if (rc != B200Q_ERR_UNSUPPORTED) return rc;
     if (elem == ELEM_F32) return pair_out<float>(p, s, dependent);
     if (elem == ELEM_F16) return pair_out<__half>(p, s, dependent);
     return pair_out<__nv_bfloat16>(p, s, dependent);

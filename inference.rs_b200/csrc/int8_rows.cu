@@ -160,16 +160,17 @@ template <typename OutT, int R, int NT, int U, int WK, int PER_SM> static cudaEr
     const long long tiles = (long long)((p.n + 16 * R - 1) / (16 * R)) * ((p.rows + 8 * NT - 1) / (8 * NT) + p.experts - 1), fit = (long long)PER_SM * runtime_info().sm_count;
     return launch_kernel(int8_rows_kernel<OutT, R, NT, U, WK, PER_SM>, dim3((unsigned)(tiles < fit ? tiles : fit), 1, 1), 32 * I8R_WARPS, int8_list_bytes(p.experts), s, dependent, p);
 }
-// Which form of the kernel takes a product; none where the tensor-core kernel of int8_pair.cu is the faster one. What decides is how many
-// 16-row tiles there are for 2368 warps, and how many tokens meet each weight. us, quantizer included, bf16, weights out of HBM (pair: the
-// tensor-core kernel):
-//   up to 8 tokens   8 warps a tile: 4096 x 1024 4.5 (4: 5.5, pair 10.8), 4096 x 4096 6.4 (4: 7.0), 14336 x 4096 13.5 (4: 16.5, pair 22.8)
+// Which form of the kernel takes a product; none where the tensor-core kernels (int8_pair.cu, int8_split.cu) are the faster ones. What
+// decides is how many 16-row tiles there are for 2368 warps, and how many tokens meet each weight. us, quantizer included, bf16, weights
+// out of HBM (tc: the tensor-core kernels):
+//   up to 8 tokens   8 warps a tile: 4096 x 1024 4.5 (4: 5.5, tc 8.2), 4096 x 4096 6.4 (4: 7.0), 14336 x 4096 13.5 (4: 16.5, tc 17.1)
 //                    4 warps:        one token through 2 of 8 experts of 4096 x 14336 68.9 (8: 72.7)
-//                    2 warps and 32 rows: 4096 x 28672 21.8 (4: 22.6, pair 24.3); 16 tokens through 8 of 128 experts of 2048 x 768 67.8
-//                    (4 warps, 16 rows: 78.2, pair 73.5). Experts with five tokens and more: pair (48 tokens through 6 of 64: 97.8, 98.5)
-//   more, 16 at once 16 rows:        16 tokens 4096 x 4096 7.2 (pair 11.1), 14336 x 4096 15.5 (pair 22.7); 64 tokens 4096 x 1024 6.4
-//                    32 rows:        32 tokens 4096 x 4096 8.8 (16 rows 9.7, pair 11.3), 14336 x 4096 21.4 (24.1, pair 23.2)
-//                    none:           16 tokens 4096 x 14336 16.5 (pair 15.2), 32 tokens 24.6 (15.5), 64 tokens 4096 x 4096 13.8 (11.5)
+//                    2 warps and 32 rows: 4096 x 28672 21.8 (4: 22.6, tc 24.3); 16 tokens through 8 of 128 experts of 2048 x 768 67.8
+//                    (4 warps, 16 rows: 78.2, tc 73.5). Experts with five tokens and more: tc (48 tokens through 6 of 64: 97.8, 98.5)
+//   more, 16 at once 16 rows:        16 tokens 4096 x 4096 7.3 (tc 10.1), 14336 x 4096 15.6 (17.2); 64 tokens 4096 x 1024 6.4 (8.3)
+//                    32 rows:        32 tokens 4096 x 4096 8.9 (16 rows 9.7, tc 10.2)
+//                    none, by groups of 16 tokens x tiles: 16 tokens 4096 x 14336 16.5 (tc 15.2), 48 tokens 4096 x 4096 13.1 (10.7), 96
+//                    tokens 4096 x 2048 13.4 (9.9); long rows sooner: 32 tokens 8192 x 4096 14.0 (12.5), 14336 x 4096 21.3 (17.3)
 enum class RowsForm { none, few_tiles, some_tiles, many_tiles, tokens16, tokens32 };
 static RowsForm rows_form(const Int8Product& p) {
     const int used = p.experts < p.rows ? p.experts : p.rows;  // experts with tokens, at most
@@ -178,7 +179,7 @@ static RowsForm rows_form(const Int8Product& p) {
     if (per <= 8 && tiles < 1536) return tiles < 512 ? RowsForm::few_tiles : RowsForm::some_tiles;
     if (per <= (p.experts > 1 ? 4 : 8)) return RowsForm::many_tiles;
     const long long groups = (per + 15) / 16 * tiles;
-    if (groups <= 512) return groups <= 256 || per <= 16 ? RowsForm::tokens16 : RowsForm::tokens32;
+    if (groups <= (p.k > 6144 ? 256 : 512)) return groups <= 256 || per <= 16 ? RowsForm::tokens16 : RowsForm::tokens32;
     return RowsForm::none;
 }
 bool int8_rows_pays(const Int8Product& p) { return rows_form(p) != RowsForm::none; }

@@ -135,6 +135,11 @@ __device__ __forceinline__ void tc_mma_f16_pair(uint32_t tmem_d, uint64_t desc_a
         : "memory");
 }
 
+// the same for a pair in a larger cluster; `pair_mask` has the bits of its two CTAs
+__device__ __forceinline__ void tc_commit_pair_to(uint64_t* bar, unsigned short pair_mask) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"(pair_mask)
+                 : "memory");
+}
 // kind::i8: 8-bit integers, 32 of a row per instruction, s32 accumulator
 __device__ __forceinline__ void tc_mma_i8_pair(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(

@@ -153,6 +153,14 @@ def test_larger_products(m, n, k):
     assert_device_ok()
 
 
+@pytest.mark.parametrize("m", [33, 64, 65, 96, 130, 161, 200, 225, 256, 300, 512])
+@pytest.mark.parametrize("n,k", [(2048, 2048), (4096, 2500), (4000, 14336), (8000, 2100), (9300, 4096)])
+def test_few_tiles_and_long_sums(m, n, k):
+    """Shapes whose tiles are few for the chip: k is divided."""
+    check_product(m, n, k, DTYPES[m % 3])
+    assert_device_ok()
+
+
 def test_the_largest_sums_are_exact():
     """131072 products of 127 and -128: 2.13e9, one bit below the end of 32."""
     k = 131072
