@@ -99,6 +99,12 @@ template <> struct Eight<float> {
         b = *(reinterpret_cast<const float4*>(p) + 1);
     }
     __device__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+    __device__ void load_some(const float* x, int c, int k) {  // of x[c..c + 8) what lies in [0, k)
+        float* v[8] = {&a.x, &a.y, &a.z, &a.w, &b.x, &b.y, &b.z, &b.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i >= 0 && c + i < k) *v[i] = x[c + i];
+    }
     static __device__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
     __device__ uint32_t top(uint32_t m) const {
         m = max(m, max(max(abs_bits(a.x), abs_bits(a.y)), max(abs_bits(a.z), abs_bits(a.w))));
@@ -115,6 +121,12 @@ template <typename T> struct Eight {
     uint4 a;
     __device__ void load(const T* p) { a = *reinterpret_cast<const uint4*>(p); }
     __device__ void zero() { a = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ void load_some(const T* x, int c, int k) {
+        uint32_t* w[4] = {&a.x, &a.y, &a.z, &a.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i >= 0 && c + i < k) *w[i / 2] |= (uint32_t)*reinterpret_cast<const unsigned short*>(x + c + i) << (16 * (i & 1));
+    }
     using Pair = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
     __device__ uint32_t top(uint32_t m) const {  // two values side by side, a NaN above all
         const Pair* w = reinterpret_cast<const Pair*>(&a);
@@ -163,16 +175,27 @@ __device__ __forceinline__ void store_scale(const QuantizeRows& p, long long row
     }
 }
 
-// `size` threads (a warp or a CTA) and their share of a row: eight values per thread and step.
-template <typename T, int STEPS> struct RowPart {
+// `size` threads (a warp or a CTA) and their share of a row: eight values per thread and step, group g of them with rank g % size.
+// ODD: a row starts anywhere. Its groups are those between 16-byte boundaries, so that the first holds `head` values of what lies before
+// (and counts them as zeros, as the last does with what lies behind; these two are read value by value), and a group's integers are
+// those of two neighbours, `head` bytes on.
+template <typename T, int STEPS, bool ODD> struct RowPart {
     Eight<T> held[STEPS];
+    int head;
     __device__ __forceinline__ void load(const QuantizeRows& p, long long row, int rank, int size) {
         const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+        head = ODD ? (int)(reinterpret_cast<uintptr_t>(x) % 16 / sizeof(T)) : 0;
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
-            const int c = 8 * (rank + i * size);
-            if (c < p.k) held[i].load(x + c);
-            else held[i].zero();
+            const int c = 8 * (rank + i * size) - head;
+            if (c >= 0 && c + 8 <= p.k) {
+                held[i].load(x + c);
+            } else {
+                held[i].zero();
+                if constexpr (ODD) {
+                    if (c < p.k) held[i].load_some(x, c, p.k);
+                }
+            }
         }
     }
     __device__ __forceinline__ uint32_t top() const {
@@ -181,54 +204,86 @@ template <typename T, int STEPS> struct RowPart {
         for (int i = 0; i < STEPS; ++i) m = held[i].top(m);
         return Eight<T>::float_bits(m);
     }
-    __device__ __forceinline__ void store(const QuantizeRows& p, long long row, const RowScale& r, int rank, int size) const {
+    // by all of the threads; `next`: of the eight integers of a group and step, those of the group behind it
+    template <typename Next> __device__ __forceinline__ void store(const QuantizeRows& p, long long row, const RowScale& r, int rank, int size, Next next) const {
         const int kp = (p.k + 15) & ~15;
         if (rank == 0) store_scale(p, row, r.s);
+        uint2 w[STEPS];
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            float v[8];
+            held[i].get(v);
+            w[i] = make_uint2(quantize_any<Eight<T>::HALVES>(v[0], v[1], v[2], v[3], r), quantize_any<Eight<T>::HALVES>(v[4], v[5], v[6], v[7], r));
+        }
+        if constexpr (ODD) next(w, head);
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
             const int c = 8 * (rank + i * size);
             if (c >= kp) break;
-            float v[8];
-            held[i].get(v);
-            const uint2 w = make_uint2(quantize_any<Eight<T>::HALVES>(v[0], v[1], v[2], v[3], r), quantize_any<Eight<T>::HALVES>(v[4], v[5], v[6], v[7], r));
             if (p.position == nullptr) {
-                *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = w;
+                *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = w[i];
             } else {
                 for (int j = 0; j < p.topk; ++j) {
                     const int to = p.position[row * p.topk + j];
-                    if (to >= 0) *reinterpret_cast<uint2*>(p.q + (long long)to * p.ldq + c) = w;
+                    if (to >= 0) *reinterpret_cast<uint2*>(p.q + (long long)to * p.ldq + c) = w[i];
                 }
             }
         }
     }
 };
+// bytes `head`.. of two groups' sixteen
+__device__ __forceinline__ uint2 shifted(uint2 a, uint2 b, int head) {
+    const bool far = head >= 4;
+    const uint32_t w0 = far ? a.y : a.x, w1 = far ? b.x : a.y, w2 = far ? b.y : b.x;
+    return make_uint2(__funnelshift_r(w0, w1, 8 * (head & 3)), __funnelshift_r(w1, w2, 8 * (head & 3)));
+}
 __device__ __forceinline__ long long row_count(const QuantizeRows& p) {
     return p.row_limit != nullptr ? min((long long)max(*p.row_limit, 0), p.rows) : p.rows;
 }
 
-// A CTA per row.
-template <typename T, int STEPS, int MAX_THREADS> __global__ void __launch_bounds__(MAX_THREADS) int8_quantize_kernel(const QuantizeRows p) {
+// A CTA per row; ODD rows pass their integers on through shared memory.
+template <typename T, int STEPS, int MAX_THREADS, bool ODD> __global__ void __launch_bounds__(MAX_THREADS) int8_quantize_kernel(const QuantizeRows p) {
+    extern __shared__ uint2 groups[];
     grid_dependency_wait();
     grid_launch_dependents();
     const long long row = blockIdx.x;
     if (row >= row_count(p)) return;
-    RowPart<T, STEPS> part;
-    part.load(p, row, threadIdx.x, blockDim.x);
-    part.store(p, row, row_scale(block_max(part.top())), threadIdx.x, blockDim.x);
+    const int rank = threadIdx.x, size = blockDim.x;
+    RowPart<T, STEPS, ODD> part;
+    part.load(p, row, rank, size);
+    part.store(p, row, row_scale(block_max(part.top())), rank, size, [&](uint2 (&w)[STEPS], int head) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) groups[rank + i * size] = w[i];
+        if (rank == 0) groups[STEPS * size] = make_uint2(0u, 0u);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) w[i] = shifted(w[i], groups[rank + i * size + 1], head);
+    });
 }
 // A warp per row, rows of up to 1024 values: a CTA for each such row would cost its start, about a nanosecond.
-template <typename T> __global__ void __launch_bounds__(256) int8_quantize_short_kernel(const QuantizeRows p) {
+template <typename T, int STEPS, bool ODD> __global__ void __launch_bounds__(256) int8_quantize_short_kernel(const QuantizeRows p) {
     grid_dependency_wait();
     grid_launch_dependents();
     const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     if (row >= row_count(p)) return;
-    RowPart<T, 4> part;
+    RowPart<T, STEPS, ODD> part;
     part.load(p, row, lane, 32);
-    part.store(p, row, row_scale(__reduce_max_sync(0xffffffffu, part.top())), lane, 32);
+    part.store(p, row, row_scale(__reduce_max_sync(0xffffffffu, part.top())), lane, 32, [&](uint2 (&w)[STEPS], int head) {
+        uint2 behind[STEPS];
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            const uint2 first = i < STEPS - 1 ? w[i + 1] : make_uint2(0u, 0u);  // lane 31's neighbour: lane 0 of the next step
+            behind[i] = make_uint2(__shfl_down_sync(0xffffffffu, w[i].x, 1), __shfl_down_sync(0xffffffffu, w[i].y, 1));
+            const uint2 wrap = make_uint2(__shfl_sync(0xffffffffu, first.x, 0), __shfl_sync(0xffffffffu, first.y, 0));
+            if (lane == 31) behind[i] = wrap;
+        }
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) w[i] = shifted(w[i], behind[i], head);
+    });
 }
 
-// Any width, any alignment of x: a value at a time, the row read twice.
+// Rows too wide to hold: a value at a time, the row read twice.
 template <typename T> __global__ void __launch_bounds__(256) int8_quantize_plain_kernel(const QuantizeRows p) {
     grid_dependency_wait();
     grid_launch_dependents();
@@ -256,17 +311,26 @@ template <typename T> __global__ void __launch_bounds__(256) int8_quantize_plain
     }
 }
 
-template <typename T> static cudaError_t quantize_t(const QuantizeRows& p, cudaStream_t s, bool dependent) {
-    const bool wide = p.k % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ldx * sizeof(T) % 16 == 0 && p.k <= 32768;
-    if (!wide) return launch_kernel(int8_quantize_plain_kernel<T>, dim3((unsigned)p.rows, 1, 1), 256, 0, s, dependent, p);
+template <typename T, bool ODD> static cudaError_t quantize_held(const QuantizeRows& p, cudaStream_t s, bool dependent) {
+    if (p.k > (ODD ? 32768 - 16 : 32768)) return launch_kernel(int8_quantize_plain_kernel<T>, dim3((unsigned)p.rows, 1, 1), 256, 0, s, dependent, p);
     const long long sms = runtime_info().sm_count;
-    const int eights = (p.k + 15) / 16 * 2, whole = (eights + 31) / 32 * 32;
+    const int eights = (p.k + 15) / 16 * 2 + (ODD ? 1 : 0), whole = (eights + 31) / 32 * 32;
+    const auto go = [&](auto kernel, unsigned threads, int steps) {
+        return launch_kernel(kernel, dim3((unsigned)p.rows, 1, 1), threads, ODD ? (threads * steps + 1) * sizeof(uint2) : 0, s, dependent, p);
+    };
     // few rows: every thread as few steps as there can be, the shortest way
-    if (p.rows <= 2 * sms && whole <= 1024) return launch_kernel(int8_quantize_kernel<T, 1, 1024>, dim3((unsigned)p.rows, 1, 1), (unsigned)whole, 0, s, dependent, p);
-    if (p.k <= 1024) return launch_kernel(int8_quantize_short_kernel<T>, dim3((unsigned)((p.rows + 7) / 8), 1, 1), 256, 0, s, dependent, p);
+    if (p.rows <= 2 * sms && whole <= 1024) return go(int8_quantize_kernel<T, 1, 1024, ODD>, (unsigned)whole, 1);
+    if (eights <= 128) {
+        const auto kernel = eights <= 32 ? int8_quantize_short_kernel<T, 1, ODD> : (eights <= 64 ? int8_quantize_short_kernel<T, 2, ODD> : int8_quantize_short_kernel<T, 4, ODD>);
+        return launch_kernel(kernel, dim3((unsigned)((p.rows + 7) / 8), 1, 1), 256, 0, s, dependent, p);
+    }
     const unsigned threads = (unsigned)((eights + 127) / 128 * 32);
-    if (threads <= 512) return launch_kernel(int8_quantize_kernel<T, 4, 512>, dim3((unsigned)p.rows, 1, 1), threads, 0, s, dependent, p);
-    return launch_kernel(int8_quantize_kernel<T, 4, 1024>, dim3((unsigned)p.rows, 1, 1), threads, 0, s, dependent, p);
+    if (threads <= 512) return go(int8_quantize_kernel<T, 4, 512, ODD>, threads, 4);
+    return go(int8_quantize_kernel<T, 4, 1024, ODD>, threads, 4);
+}
+template <typename T> static cudaError_t quantize_t(const QuantizeRows& p, cudaStream_t s, bool dependent) {
+    const bool odd = p.k % 8 != 0 || reinterpret_cast<uintptr_t>(p.x) % 16 != 0 || p.ldx * sizeof(T) % 16 != 0;
+    return odd ? quantize_held<T, true>(p, s, dependent) : quantize_held<T, false>(p, s, dependent);
 }
 
 cudaError_t int8_quantize_rows(int elem, const void* x, long long ldx, int8_t* q, long long ldq, float* scales, long long rows, int k,
@@ -277,33 +341,41 @@ cudaError_t int8_quantize_rows(int elem, const void* x, long long ldx, int8_t* q
     return quantize_t<__nv_bfloat16>(p, s, dependent);
 }
 
-// V values per thread and step, one 16-byte store (two of them side by side per lane left the sectors half written: f32, 14336 x 4096 55 us).
-template <typename T, int V> __global__ void __launch_bounds__(256) int8_dequantize_kernel(const int8_t* __restrict__ q, long long ldq, const float* __restrict__ scales,
-                                                                                           T* __restrict__ out, int k) {
-    const long long row = blockIdx.x;
+// 16 bytes of values per thread and step, one store: a row's groups are those between 16-byte boundaries of the output, and their integers
+// are shifted out of aligned words. ODD: rows start anywhere, and their first and last groups are written value by value. SIZE threads
+// per row, so that short rows share a CTA. (Two stores side by side per lane, which leave every sector half written: f32, 14336 x 4096,
+// 55 us against 46.)
+template <typename T, int SIZE, bool ODD> __global__ void __launch_bounds__(256) int8_dequantize_kernel(const int8_t* __restrict__ q, long long ldq, const float* __restrict__ scales,
+                                                                                              T* __restrict__ out, long long rows, int k) {
+    constexpr int V = 16 / sizeof(T);
+    const long long row = (long long)blockIdx.x * (256 / SIZE) + threadIdx.x / SIZE;
+    if (row >= rows) return;
     const float s = scales[row];
     const int8_t* src = q + row * ldq;
     T* dst = out + row * k;
-    if constexpr (V > 1) {
+    const int head = ODD ? (int)(reinterpret_cast<uintptr_t>(dst) % 16 / sizeof(T)) : 0, shift = 8 * (-head & 3);
 #pragma unroll 4
-        for (int c = V * threadIdx.x; c < k; c += V * 256) {
-            uint32_t w[V / 4];
-            if constexpr (V == 8) *reinterpret_cast<uint2*>(w) = __ldg(reinterpret_cast<const uint2*>(src + c));
-            else w[0] = __ldg(reinterpret_cast<const uint32_t*>(src + c));
+    for (int c = V * (int)(threadIdx.x % SIZE) - head; c < k; c += V * SIZE) {
+        if (!ODD || (c >= 0 && c + V <= k)) {
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(src + (c & ~3));
+            uint32_t b[V / 4 + 1];
+#pragma unroll
+            for (int j = 0; j < V / 4; ++j) b[j] = __ldg(w + j);
+            b[V / 4] = ODD && shift != 0 ? __ldg(w + V / 4) : 0u;
             alignas(16) T v[V];
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = from_float<T>((float)(int8_t)(w[j / 4] >> (8 * (j % 4))) * s);
+            for (int j = 0; j < V; ++j) v[j] = from_float<T>((float)(int8_t)(__funnelshift_r(b[j / 4], b[j / 4 + 1], shift) >> (8 * (j % 4))) * s);
             *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(v);
+        } else {
+            for (int j = max(0, -c); j < min(V, k - c); ++j) dst[c + j] = from_float<T>((float)src[c + j] * s);
         }
-    } else {
-        for (int c = threadIdx.x; c < k; c += 256) dst[c] = from_float<T>((float)src[c] * s);
     }
 }
 template <typename T> static cudaError_t dequantize_t(const int8_t* q, long long ldq, const float* scales, void* out, long long rows, int k, cudaStream_t s) {
-    constexpr int V = 16 / sizeof(T);
-    const bool wide = k % V == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0;
-    const auto kernel = wide ? int8_dequantize_kernel<T, V> : int8_dequantize_kernel<T, 1>;
-    return launch_kernel(kernel, dim3((unsigned)rows, 1, 1), 256, 0, s, false, q, ldq, scales, static_cast<T*>(out), k);
+    const bool shared = k <= 1024, odd = reinterpret_cast<uintptr_t>(out) % 16 != 0 || k % (16 / sizeof(T)) != 0;
+    const auto kernel = odd ? (shared ? int8_dequantize_kernel<T, 32, true> : int8_dequantize_kernel<T, 256, true>)
+                            : (shared ? int8_dequantize_kernel<T, 32, false> : int8_dequantize_kernel<T, 256, false>);
+    return launch_kernel(kernel, dim3((unsigned)(shared ? (rows + 7) / 8 : rows), 1, 1), 256, 0, s, false, q, ldq, scales, static_cast<T*>(out), rows, k);
 }
 
 cudaError_t int8_dequantize_rows(int elem, const int8_t* q, long long ldq, const float* scales, void* out, long long rows, int k, cudaStream_t s) {

@@ -78,31 +78,37 @@ cudaError_t route_sort(const void* ids, bool wide, int slots, int experts, int* 
     return launch_kernel(route_sort_kernel<int>, grid, RT_THREADS, 0, s, false, static_cast<const int*>(ids), slots, experts, order, offsets, position);
 }
 
-// V neighbouring values of a row as they lie in memory: 1, or 4 or 8, as many as fill the 16 bytes of a store (two half-filled stores per
-// lane would leave every sector half written)
-template <typename T, int V> struct Values {
-    alignas(V == 1 ? sizeof(T) : (V * sizeof(T) >= 16 ? 16 : 8)) T raw[V];
-    __device__ __forceinline__ void load(const T* p) {
-        if constexpr (V == 1) {
-            raw[0] = *p;
+// A thread's values of a row as they lie in memory. WIDE: V neighbouring ones from column c on, as many as fill the 16 bytes of a store
+// (two half-filled stores per lane would leave every sector half written). Otherwise, for rows at any alignment, columns c, c + step, ...:
+// a warp's loads are still neighbouring values, and V of them are under way per thread.
+template <typename T, int V, bool WIDE> struct Values {
+    alignas(WIDE ? (V * sizeof(T) >= 16 ? 16 : 8) : sizeof(T)) T raw[V];
+    __device__ __forceinline__ void load(const T* row, int c, int step, int h) {
+        if constexpr (!WIDE) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) raw[i] = c + i * step < h ? row[c + i * step] : from_float<T>(0.0f);
         } else if constexpr (V * sizeof(T) == 8) {
-            *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(p);
+            *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(row + c);
         } else {
 #pragma unroll
-            for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(raw)[i] = *(reinterpret_cast<const uint4*>(p) + i);
+            for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(raw)[i] = *(reinterpret_cast<const uint4*>(row + c) + i);
         }
     }
-    __device__ __forceinline__ void store(T* p) const {
-        if constexpr (V == 1) {
-            *p = raw[0];
+    __device__ __forceinline__ void store(T* row, int c, int step, int h) const {
+        if constexpr (!WIDE) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (c + i * step < h) row[c + i * step] = raw[i];
         } else {  // (never less than 16 bytes)
 #pragma unroll
-            for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(raw)[i];
+            for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i) reinterpret_cast<uint4*>(row + c)[i] = reinterpret_cast<const uint4*>(raw)[i];
         }
     }
     __device__ __forceinline__ float get(int i) const { return to_float<T>(raw[i]); }
     __device__ __forceinline__ void set(int i, float v) { raw[i] = from_float<T>(v); }
 };
+// the first column of a thread's loop over a row
+template <int V, bool WIDE> __device__ __forceinline__ int first_column() { return WIDE ? V * threadIdx.x : threadIdx.x; }
 static bool rows_wide(const void* p, long long ld, int elem) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * (elem == ELEM_F32 ? 4 : 2) % 16 == 0;
 }
@@ -152,12 +158,13 @@ cudaError_t route_dispatch(int elem, const void* x, long long ldx, const int* po
     };
     if (rows_wide(x, ldx, elem) && rows_wide(rows, h, elem)) return go(uint4{}, 16 / es);
     if (es == 4) return go(uint32_t{}, 1);
+    if (reinterpret_cast<uintptr_t>(x) % 4 == 0 && reinterpret_cast<uintptr_t>(rows) % 4 == 0 && ldx % 2 == 0 && h % 2 == 0) return go(uint32_t{}, 2);
     return go(uint16_t{}, 1);
 }
 
 // out[t] = sum_j weights[t, j] rows[position[t, j]]; weights null: 1. The loads of four slots' rows are under way at once: one after the
 // other, eight slots of seven tokens took 7.4 us.
-template <typename In, typename Out, int V, int S>
+template <typename In, typename Out, int V, int S, bool WIDE>
 __global__ void __launch_bounds__(RT_ROW_THREADS) route_combine_kernel(const In* rows, long long ldr, const int* position, const float* weights, Out* out, int topk,
                                                             int h) {
     grid_dependency_wait();
@@ -172,14 +179,14 @@ __global__ void __launch_bounds__(RT_ROW_THREADS) route_combine_kernel(const In*
         for (int i = 0; i < S; ++i) w[i] = weights == nullptr ? 1.0f : (j + i < topk ? weights[t * topk + j + i] : 0.0f);
     };
     slots(0);
-    for (int c = V * threadIdx.x; c < h; c += V * blockDim.x) {
+    for (int c = first_column<V, WIDE>(); c < h; c += V * blockDim.x) {
         float sum[V] = {};
         for (int j = 0; j < topk; j += S) {
             if (topk > S) slots(j);
-            Values<In, V> r[S];
+            Values<In, V, WIDE> r[S];
 #pragma unroll
             for (int i = 0; i < S; ++i)
-                if (p[i] >= 0) r[i].load(rows + p[i] * ldr + c);
+                if (p[i] >= 0) r[i].load(rows + p[i] * ldr, c, blockDim.x, h);
 #pragma unroll
             for (int i = 0; i < S; ++i)
                 if (p[i] >= 0) {
@@ -187,10 +194,10 @@ __global__ void __launch_bounds__(RT_ROW_THREADS) route_combine_kernel(const In*
                     for (int k = 0; k < V; ++k) sum[k] = fmaf(w[i], r[i].get(k), sum[k]);
                 }
         }
-        Values<Out, V> v;
+        Values<Out, V, WIDE> v;
 #pragma unroll
         for (int k = 0; k < V; ++k) v.set(k, sum[k]);
-        v.store(out + t * h + c);
+        v.store(out + t * h, c, blockDim.x, h);
     }
 }
 
@@ -199,8 +206,8 @@ static cudaError_t combine_t(bool wide, const void* rows, long long ldr, const i
                              int h, cudaStream_t s, bool dependent) {
     const dim3 grid((unsigned)tokens, 1, 1);
     constexpr int V = 16 / sizeof(Out);
-    const auto kernel = wide ? (topk <= 2 ? route_combine_kernel<In, Out, V, 2> : route_combine_kernel<In, Out, V, 4>) : route_combine_kernel<In, Out, 1, 4>;
-    return launch_kernel(kernel, grid, row_threads(wide ? h / V : h), 0, s, dependent, static_cast<const In*>(rows), ldr, position, weights, static_cast<Out*>(out), topk, h);
+    const auto kernel = wide ? (topk <= 2 ? route_combine_kernel<In, Out, V, 2, true> : route_combine_kernel<In, Out, V, 4, true>) : route_combine_kernel<In, Out, 4, 4, false>;
+    return launch_kernel(kernel, grid, row_threads(wide ? h / V : (h + 3) / 4), 0, s, dependent, static_cast<const In*>(rows), ldr, position, weights, static_cast<Out*>(out), topk, h);
 }
 cudaError_t route_combine(int elem_in, int elem_out, const void* rows, long long ldr, const int* position, const float* weights, void* out,
                           int tokens, int topk, int h, cudaStream_t s, bool dependent) {
@@ -222,7 +229,7 @@ cudaError_t route_combine(int elem_in, int elem_out, const void* rows, long long
 
 // The gradients of combine, a CTA per token: its slots' rows of drows (each written by one CTA), and the products with the rows, four
 // slots at a time. Rows behind the last become zeros as in dispatch. Either output may be left out (null).
-template <typename G, typename T, int V, int S>
+template <typename G, typename T, int V, int S, bool WIDE>
 __global__ void __launch_bounds__(RT_ROW_THREADS) route_combine_grad_kernel(const G* __restrict__ grad_out, long long ldg, const T* __restrict__ rows, long long ldr,
                                                                  const int* __restrict__ position, const int* __restrict__ valid,
                                                                  const float* __restrict__ weights, T* __restrict__ grad_rows,
@@ -236,14 +243,14 @@ __global__ void __launch_bounds__(RT_ROW_THREADS) route_combine_grad_kernel(cons
         float w[S], dot[S] = {};
 #pragma unroll
         for (int i = 0; i < S; ++i) w[i] = j + i < topk ? weights[t * topk + j + i] : 0.0f;
-        for (int c = V * threadIdx.x; c < h; c += V * blockDim.x) {
-            Values<G, V> g;
-            g.load(grad_out + t * ldg + c);
+        for (int c = first_column<V, WIDE>(); c < h; c += V * blockDim.x) {
+            Values<G, V, WIDE> g;
+            g.load(grad_out + t * ldg, c, blockDim.x, h);
             if (grad_weights != nullptr) {
-                Values<T, V> r[S];
+                Values<T, V, WIDE> r[S];
 #pragma unroll
                 for (int i = 0; i < S; ++i)
-                    if (p[i] >= 0) r[i].load(rows + p[i] * ldr + c);
+                    if (p[i] >= 0) r[i].load(rows + p[i] * ldr, c, blockDim.x, h);
 #pragma unroll
                 for (int i = 0; i < S; ++i)
                     if (p[i] >= 0) {
@@ -254,16 +261,16 @@ __global__ void __launch_bounds__(RT_ROW_THREADS) route_combine_grad_kernel(cons
             if (grad_rows != nullptr) {
 #pragma unroll
                 for (int i = 0; i < S; ++i) {
-                    Values<T, V> d;
+                    Values<T, V, WIDE> d;
                     if (p[i] >= 0) {
 #pragma unroll
                         for (int k = 0; k < V; ++k) d.set(k, w[i] * g.get(k));
-                        d.store(grad_rows + (long long)p[i] * h + c);
+                        d.store(grad_rows + (long long)p[i] * h, c, blockDim.x, h);
                     }
                     if (j + i < topk && t * topk + j + i >= nvalid) {
 #pragma unroll
                         for (int k = 0; k < V; ++k) d.set(k, 0.0f);
-                        d.store(grad_rows + (t * topk + j + i) * h + c);
+                        d.store(grad_rows + (t * topk + j + i) * h, c, blockDim.x, h);
                     }
                 }
             }
@@ -293,8 +300,8 @@ static cudaError_t combine_grad_t(bool wide, const void* grad_out, long long ldg
     const T* r = static_cast<const T*>(rows);
     T* d = static_cast<T*>(grad_rows);
     constexpr int V = 16 / sizeof(T);
-    const auto kernel = wide ? (topk <= 2 ? route_combine_grad_kernel<G, T, V, 2> : route_combine_grad_kernel<G, T, V, 4>) : route_combine_grad_kernel<G, T, 1, 4>;
-    return launch_kernel(kernel, grid, h >= 8 ? row_threads(wide ? h / V : h) : 32u, 0, s, false, g, ldg, r, ldr, position, valid, weights, d, grad_weights, topk, h);
+    const auto kernel = wide ? (topk <= 2 ? route_combine_grad_kernel<G, T, V, 2, true> : route_combine_grad_kernel<G, T, V, 4, true>) : route_combine_grad_kernel<G, T, 4, 4, false>;
+    return launch_kernel(kernel, grid, h >= 8 ? row_threads(wide ? h / V : (h + 3) / 4) : 32u, 0, s, false, g, ldg, r, ldr, position, valid, weights, d, grad_weights, topk, h);
 }
 cudaError_t route_combine_grad(int elem_grad, int elem, const void* grad_out, long long ldg, const void* rows, long long ldr, const int* position,
                                const int* valid, const float* weights, void* grad_rows, float* grad_weights, int tokens, int topk, int h,

@@ -84,11 +84,13 @@ def test_quantize_is_the_definition(m, k, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_quantize_of_strided_and_unaligned_rows(dtype):
-    big = acts(9, 300, dtype)
-    for x in (big[:, :256], big[:, 1:257], big[::2, 3:40], big.t(), big[:, :1], big[4:5, 8:264]):
+    big, wide, many = acts(9, 300, dtype), acts(6, 9000, dtype), acts(700, 1100, dtype)
+    parts = [big[:, i:i + n] for i in range(9) for n in (1, 7, 8, 9, 15, 16, 17, 250)]
+    parts += [wide[:, i:i + n] for i in (0, 1, 5) for n in (2049, 4095, 8193)] + [many[:, i:i + n] for i in (0, 3, 8) for n in (900, 1007, 1024, 1025, 1099 - i)]
+    for x in (*parts, big[:, :256], big[:, 1:257], big[::2, 3:40], big.t(), big[:, :1], big[4:5, 8:264], acts(3, 32751, dtype), acts(2, 32761, dtype)):
         want_q, want_s = rows64(x)
         q, s = ops.int8_quantize(x)
-        assert torch.equal(q[:, :x.shape[1]].double(), want_q) and torch.equal(s, want_s)
+        assert torch.equal(q[:, :x.shape[1]].double(), want_q) and torch.equal(s, want_s) and not q[:, x.shape[1]:].any(), tuple(x.shape)
 
 
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
