@@ -57,10 +57,11 @@ static ExpertsWorkspace experts_workspace(void* base, int elem, long long slots,
     w.position = static_cast<int*>(take(slots * 4));
     w.xs = static_cast<float*>(take(slots * 4));
     w.hs = static_cast<float*>(take(slots * 4));
-    w.xq = static_cast<int8_t*>(take(slots * w.ldx));
-    w.hidden = take(slots * w.ldh * (elem == ELEM_F32 ? 4 : 2));
-    w.hq = static_cast<int8_t*>(take(slots * w.ldh));
-    w.y = static_cast<float*>(take(slots * w.ldy * 4));
+    // the tokens' integers are done with when the hidden values' are written, and these when the outputs are
+    const long long hidden_bytes = w.ldh * (elem == ELEM_F32 ? 4 : 2), y_bytes = w.ldy * 4;
+    w.xq = w.hq = static_cast<int8_t*>(take(slots * (w.ldx > w.ldh ? w.ldx : w.ldh)));
+    w.hidden = take(slots * (hidden_bytes > y_bytes ? hidden_bytes : y_bytes));
+    w.y = static_cast<float*>(w.hidden);
     w.bytes = used;
     return w;
 }
