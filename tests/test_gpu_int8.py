@@ -83,6 +83,19 @@ def test_quantize_is_the_definition(m, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_the_smallest_numbers(dtype):
+    g = torch.Generator(device="cuda").manual_seed(4)
+    tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps  # the step of the subnormals
+    x = (torch.randint(-130, 131, (6, 300), device="cuda", generator=g).double() * tiny).to(dtype)
+    x[1] *= 0
+    x[2, 1:] = 0
+    x[3] *= 100
+    want_q, want_s = rows64(x)
+    t = pkg.Int8Tensor.quantize(x)
+    assert torch.equal(t.scales, want_s) and torch.equal(t.data[:, :300].double(), want_q)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_quantize_of_strided_and_unaligned_rows(dtype):
     big, wide, many = acts(9, 300, dtype), acts(6, 9000, dtype), acts(700, 1100, dtype)
     parts = [big[:, i:i + n] for i in range(9) for n in (1, 7, 8, 9, 15, 16, 17, 250)]
