@@ -397,7 +397,7 @@ int b200q_int8_quantize(int elem, const void* x, long long ldx, void* q, long lo
                         void* stream);
 int b200q_int8_dequantize(int elem, const void* q, long long ldq, const float* scales, void* out, long long rows, int k, void* stream);
 
-/* y[r][i] = (sum_k xq[r][k] wq[e][i][k]) * xs[r] * ws[e][i], the sum an exact integer (k at most 131072), the rest in f32,
+/* y[r][i] = (sum_k xq[r][k] wq[e][i][k]) * xs[r] * ws[e][i], the sum an exact integer (k at most 131071), the rest in f32,
  * y of element type `elem`. Several matrices wq [experts][n] and scales ws [experts][n]: rows offsets[e] .. offsets[e + 1]
  * belong to matrix e (offsets: experts + 1 device ints that do not fall, the last at most `rows`); rows of y behind
  * offsets[experts] are left as they are. One matrix with all rows: experts 1, offsets null. */

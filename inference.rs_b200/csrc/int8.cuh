@@ -8,8 +8,8 @@ namespace b200q {
 
 int set_error(int code, const char* msg);
 
-// Sums of K products of at most 128 * 127 stay inside 32 bits up to here.
-constexpr int INT8_MAX_K = 131072;
+// Sums of K products of at most 128 * 128 stay inside 32 bits up to here.
+constexpr int INT8_MAX_K = 131071;
 constexpr int INT8_MAX_EXPERTS = 1024;
 
 // Activation of a gated product, act(gate) * up, by the ids of the reference's host side

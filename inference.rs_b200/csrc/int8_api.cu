@@ -17,7 +17,7 @@ static int check_int8_rows(const void* q, long long ldq, int k, const char* what
 }
 static int check_k(int k) {
     if (k < 1) return set_error(B200Q_ERR_INVALID, "k must be positive");
-    if (k > INT8_MAX_K) return set_error(B200Q_ERR_UNSUPPORTED, "sums of more than 131072 int8 products do not fit 32 bits");
+    if (k > INT8_MAX_K) return set_error(B200Q_ERR_UNSUPPORTED, "sums of more than 131071 int8 products do not fit 32 bits");
     return B200Q_OK;
 }
 static int check_routing(long long tokens, int topk, int experts) {

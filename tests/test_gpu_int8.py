@@ -161,8 +161,8 @@ def test_products(m, n, k):
     assert_device_ok()
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 1024, 4096), (4, 64, 20000), (16, 4096, 14336), (40, 6144, 130), (333, 6144, 4096), (1500, 2000, 3008), (2, 16, 131072),
-                                   (300, 16, 131072)])
+@pytest.mark.parametrize("m,n,k", [(1, 1024, 4096), (4, 64, 20000), (16, 4096, 14336), (40, 6144, 130), (333, 6144, 4096), (1500, 2000, 3008), (2, 16, 131071),
+                                   (300, 16, 131071)])
 def test_larger_products(m, n, k):
     check_product(m, n, k, torch.bfloat16)
     assert_device_ok()
@@ -177,12 +177,13 @@ def test_few_tiles_and_long_sums(m, n, k):
 
 
 def test_the_largest_sums_are_exact():
-    """131072 products of 127 and -128: 2.13e9, one bit below the end of 32."""
-    k = 131072
+    """131071 products of -128 and -128: 2^31 - 16384."""
+    k = 131071
     w = pkg.Int8Tensor(torch.full((40, k), -128, dtype=torch.int8, device="cuda"), torch.ones(40, device="cuda"))
-    for m in (1, 130):
-        y = ops.int8_gemm(torch.full((m, k), 127, dtype=torch.int8, device="cuda"), torch.ones(m, device="cuda"), w.data, w.scales, k, torch.float32)
-        assert (y == -128.0 * 127 * k).all()
+    for m in (1, 30, 130, 600):
+        x = pkg.Int8Tensor(torch.full((m, k), -128, dtype=torch.int8, device="cuda"), torch.ones(m, device="cuda"))
+        y = ops.int8_gemm(x.data, x.scales, w.data, w.scales, k, torch.float32)
+        assert (y.double() == 2.0 ** 31 - 2 ** 14).all()  # (17 bits)
 
 
 def test_rows_of_a_batch_are_independent_and_strides_do_not_matter():
@@ -210,7 +211,7 @@ def test_outputs_and_weights_beyond_32_bit_offsets():
     xq, xs = rows64(x[-70:])
     close(y[-70:], (xq @ w.data.double().T) * xs.double()[:, None] * w.scales.double())
     del y
-    n, k = 18000, 131072  # 2.36e9 bytes of weights
+    n, k = 18000, 131056  # 2.36e9 bytes of weights
     data = torch.zeros(n, k, dtype=torch.int8, device="cuda")
     data[-100:] = torch.randint(-128, 128, (100, k), dtype=torch.int8, device="cuda")
     w = pkg.Int8Tensor(data, torch.ones(n, device="cuda"))
@@ -233,8 +234,15 @@ def test_other_streams_and_graphs(m):
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         got = [lin(v) for v in x]
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    both = []
+    for i in range(12):  # two streams at once, on the same weights
+        with torch.cuda.stream(side if i % 2 else other):
+            both.append(lin(x[i % 3]))
     side.synchronize()
-    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    other.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(y, want[i % 3]) for i, y in enumerate(both))
     # two graphs, replayed in turn: each has a workspace of its own
     buf = [x[0].clone(), x[1].clone()]
     graphs, outs = [], []
@@ -323,8 +331,8 @@ def test_product_refusals():
         ops.int8_gemm(xq, xs, w.data[0], w.scales[0], 32, torch.int32)
     with pytest.raises(ValueError, match="CUDA"):
         ops.int8_matmul(x, w.data[0].cpu(), w.scales[0])
-    with pytest.raises(pkg.KernelLibraryError, match="131072"):
-        ops.int8_quantize(torch.zeros(1, 131073, device="cuda"))
+    with pytest.raises(pkg.KernelLibraryError, match="131071"):
+        ops.int8_quantize(torch.zeros(1, 131072, device="cuda"))
 
 
 # ---- the layer of experts -------------------------------------------------------------------------------------------------

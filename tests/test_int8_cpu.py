@@ -83,7 +83,7 @@ def test_the_library_refuses_what_it_cannot_take():
     err = lambda: lib.b200q_last_error().decode()
     assert lib.b200q_int8_quantize(7, 1, 16, 16, 16, 16, 1, 16, None) == -1
     assert lib.b200q_int8_quantize(0, 16, 16, 16, 24, 16, 1, 16, None) == -2 and "16" in err()
-    assert lib.b200q_int8_quantize(0, 16, 16, 16, 16, 16, 1, 131073, None) == -1 and "131072" in err()
+    assert lib.b200q_int8_quantize(0, 16, 16, 16, 16, 16, 1, 131072, None) == -1 and "131071" in err()
     assert lib.b200q_int8_quantize(0, None, 16, None, 16, None, 0, 16, None) == 0
     assert lib.b200q_int8_matmul(0, 16, 16, 16, 16, 4, 4, 16, 16, 16, 4, 256, 8, None) == -4
     assert lib.b200q_int8_matmul(0, 16, 16, 16, 16, 4, 4, 16, 16, 16, 4, 257, 1 << 20, None) == -2
