@@ -145,6 +145,9 @@ static cudaError_t launch_kernel(Kern kernel, dim3 grid, unsigned block, size_t 
 // int8_quantize.cu
 cudaError_t int8_quantize_rows(int elem, const void* x, long long ldx, int8_t* q, long long ldq, float* scales, long long rows, int k,
                                const int* position, int topk, const int* row_limit, cudaStream_t s, bool dependent);
+bool int8_routes_quantizing(int tokens, int topk, int k);
+cudaError_t int8_route_quantize(int elem, const void* x, long long ldx, int8_t* q, long long ldq, float* scales, int tokens, int k, const void* ids,
+                                bool wide_ids, int topk, int experts, int* position, int* offsets, cudaStream_t s);
 cudaError_t int8_dequantize_rows(int elem, const int8_t* q, long long ldq, const float* scales, void* out, long long rows, int k, cudaStream_t s);
 // int8_rows.cu
 bool int8_rows_pays(const Int8Product& p);

@@ -200,8 +200,12 @@ int b200q_int8_experts(int elem, int activation, const void* x, long long ldx, c
     cudaStream_t s = (cudaStream_t)stream;
     const Int8Product up{w.xq, w.xs, static_cast<const int8_t*>(gate_up), gate_up_scales, w.hidden, w.offsets, slots, 2 * pairs, hidden, (int)w.ldx, (int)w.ldx, experts, activation, ffn, w.ldh, status_ptr()};
     const Int8Product dn{w.hq, w.hs, static_cast<const int8_t*>(down), down_scales, w.y, w.offsets, slots, hidden, ffn, (int)w.ldh, (int)w.ldh, experts, INT8_ACT_NONE, hidden, w.ldy, status_ptr()};
-    if (const int rc = cuda_result(route_sort(ids, id_bytes == 8, slots, experts, w.order, w.offsets, w.position, s))) return rc;
-    if (const int rc = cuda_result(int8_quantize_rows(elem, x, ldx, w.xq, w.ldx, w.xs, tokens, hidden, w.position, topk, nullptr, s, true))) return rc;
+    if (int8_routes_quantizing(tokens, topk, hidden)) {
+        if (const int rc = cuda_result(int8_route_quantize(elem, x, ldx, w.xq, w.ldx, w.xs, tokens, hidden, ids, id_bytes == 8, topk, experts, w.position, w.offsets, s))) return rc;
+    } else {
+        if (const int rc = cuda_result(route_sort(ids, id_bytes == 8, slots, experts, w.order, w.offsets, w.position, s))) return rc;
+        if (const int rc = cuda_result(int8_quantize_rows(elem, x, ldx, w.xq, w.ldx, w.xs, tokens, hidden, w.position, topk, nullptr, s, true))) return rc;
+    }
     if (const int rc = int8_product(elem, up, s, true)) return rc;
     if (const int rc = cuda_result(int8_quantize_rows(elem, w.hidden, w.ldh, w.hq, w.ldh, w.hs, slots, ffn, nullptr, 1, w.offsets + experts, s, true))) return rc;
     if (const int rc = int8_product(ELEM_F32, dn, s, true)) return rc;

@@ -27,6 +27,11 @@ struct QuantizeRows {
     const int* position;  // where a row's copies go: rows position[r * topk ...] of q, none for -1; null: row r
     int topk;
     const int* row_limit;  // rows from here on are left alone (null: none)
+    // routing in the same launch (int8_route_quantize): the slots' expert ids, and what route_sort would make of them
+    const void* ids;
+    bool wide_ids;
+    int experts;
+    int *position_out, *offsets;
 };
 
 constexpr float ROUND = 12582912.0f;  // 1.5 * 2^23: v + ROUND has the integer next to v in its low bits
@@ -164,16 +169,16 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v) {
     return __reduce_max_sync(0xffffffffu, w);
 }
 
-__device__ __forceinline__ void store_scale(const QuantizeRows& p, long long row, float s) {
-    if (p.position == nullptr) {
-        p.scales[row] = s;
+// The rows of q that a row goes to: itself (to null), or those of `to` that are there.
+template <typename Fn> __device__ __forceinline__ void each_target(const QuantizeRows& p, long long row, const int* to, Fn fn) {
+    if (to == nullptr) {
+        fn(row);
     } else {
-        for (int j = 0; j < p.topk; ++j) {
-            const int to = p.position[row * p.topk + j];
-            if (to >= 0) p.scales[to] = s;
-        }
+        for (int j = 0; j < p.topk; ++j)
+            if (to[j] >= 0) fn((long long)to[j]);
     }
 }
+__device__ __forceinline__ const int* targets(const QuantizeRows& p, long long row) { return p.position != nullptr ? p.position + row * p.topk : nullptr; }
 
 // `size` threads (a warp or a CTA) and their share of a row: eight values per thread and step, group g of them with rank g % size.
 // ODD: a row starts anywhere. Its groups are those between 16-byte boundaries, so that the first holds `head` values of what lies before
@@ -205,9 +210,9 @@ template <typename T, int STEPS, bool ODD> struct RowPart {
         return Eight<T>::float_bits(m);
     }
     // by all of the threads; `next`: of the eight integers of a group and step, those of the group behind it
-    template <typename Next> __device__ __forceinline__ void store(const QuantizeRows& p, long long row, const RowScale& r, int rank, int size, Next next) const {
+    template <typename Next> __device__ __forceinline__ void store(const QuantizeRows& p, long long row, const RowScale& r, int rank, int size, const int* to, Next next) const {
         const int kp = (p.k + 15) & ~15;
-        if (rank == 0) store_scale(p, row, r.s);
+        if (rank == 0) each_target(p, row, to, [&](long long at) { p.scales[at] = r.s; });
         uint2 w[STEPS];
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
@@ -220,14 +225,7 @@ template <typename T, int STEPS, bool ODD> struct RowPart {
         for (int i = 0; i < STEPS; ++i) {
             const int c = 8 * (rank + i * size);
             if (c >= kp) break;
-            if (p.position == nullptr) {
-                *reinterpret_cast<uint2*>(p.q + row * p.ldq + c) = w[i];
-            } else {
-                for (int j = 0; j < p.topk; ++j) {
-                    const int to = p.position[row * p.topk + j];
-                    if (to >= 0) *reinterpret_cast<uint2*>(p.q + (long long)to * p.ldq + c) = w[i];
-                }
-            }
+            each_target(p, row, to, [&](long long at) { *reinterpret_cast<uint2*>(p.q + at * p.ldq + c) = w[i]; });
         }
     }
 };
@@ -241,17 +239,79 @@ __device__ __forceinline__ long long row_count(const QuantizeRows& p) {
     return p.row_limit != nullptr ? min((long long)max(*p.row_limit, 0), p.rows) : p.rows;
 }
 
-// A CTA per row; ODD rows pass their integers on through shared memory.
-template <typename T, int STEPS, int MAX_THREADS, bool ODD> __global__ void __launch_bounds__(MAX_THREADS) int8_quantize_kernel(const QuantizeRows p) {
+// Routing for few slots, without a launch of its own: the CTA of a token counts through all ids where its own slots go, and one more CTA
+// finds where the experts' rows begin. What route_sort_kernel would give, in the same order.
+constexpr int ROUTE_MOST_SLOTS = 2048, ROUTE_MOST_TOPK = 8;
+__device__ __forceinline__ int expert_id(const QuantizeRows& p, int slot) {  // `experts`: of none
+    const long long id = p.wide_ids ? static_cast<const long long*>(p.ids)[slot] : static_cast<const int*>(p.ids)[slot];
+    return id >= 0 && id < p.experts ? (int)id : p.experts;
+}
+__device__ __forceinline__ void route_token(const QuantizeRows& p, int token, int (&to)[ROUTE_MOST_TOPK]) {
+    const int slots = (int)p.rows * p.topk, first = token * p.topk;
+    int mine[ROUTE_MOST_TOPK], before[ROUTE_MOST_TOPK] = {};
+#pragma unroll
+    for (int j = 0; j < ROUTE_MOST_TOPK; ++j) mine[j] = j < p.topk ? expert_id(p, first + j) : -1;
+    if (threadIdx.x < ROUTE_MOST_TOPK) to[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < slots; i += blockDim.x) {
+        const int id = expert_id(p, i);
+#pragma unroll
+        for (int j = 0; j < ROUTE_MOST_TOPK; ++j) before[j] += id < mine[j] || (id == mine[j] && i < first + j);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ROUTE_MOST_TOPK; ++j) {
+        if (j >= p.topk) break;
+        const int sum = __reduce_add_sync(0xffffffffu, before[j]);
+        if ((threadIdx.x & 31) == 0 && sum != 0) atomicAdd(&to[j], sum);  // (integers: any order)
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < p.topk) {
+        if (expert_id(p, first + threadIdx.x) == p.experts) to[threadIdx.x] = -1;
+        p.position_out[first + threadIdx.x] = to[threadIdx.x];
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void route_offsets(const QuantizeRows& p, int (&count)[INT8_MAX_EXPERTS + 1]) {
+    for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) count[e] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < (int)p.rows * p.topk; i += blockDim.x) atomicAdd(&count[expert_id(p, i)], 1);
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    int sum = 0;
+    for (int e0 = 0; e0 <= p.experts; e0 += 32) {
+        const int e = e0 + threadIdx.x, c = e < p.experts ? count[e] : 0;
+        int upto = c;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, d);
+            if ((int)threadIdx.x >= d) upto += v;
+        }
+        if (e <= p.experts) p.offsets[e] = sum + upto - c;
+        sum += __shfl_sync(0xffffffffu, upto, 31);
+    }
+}
+
+// A CTA per row; ODD rows pass their integers on through shared memory. ROUTE: see above.
+template <typename T, int STEPS, int MAX_THREADS, bool ODD, bool ROUTE> __global__ void __launch_bounds__(MAX_THREADS) int8_quantize_kernel(const QuantizeRows p) {
     extern __shared__ uint2 groups[];
+    __shared__ int to[ROUTE ? ROUTE_MOST_TOPK : 1];
     grid_dependency_wait();
     grid_launch_dependents();
     const long long row = blockIdx.x;
-    if (row >= row_count(p)) return;
+    if constexpr (ROUTE) {
+        __shared__ int count[INT8_MAX_EXPERTS + 1];
+        if (row == p.rows) {
+            route_offsets(p, count);
+            return;
+        }
+    } else {
+        if (row >= row_count(p)) return;
+    }
     const int rank = threadIdx.x, size = blockDim.x;
     RowPart<T, STEPS, ODD> part;
     part.load(p, row, rank, size);
-    part.store(p, row, row_scale(block_max(part.top())), rank, size, [&](uint2 (&w)[STEPS], int head) {
+    if constexpr (ROUTE) route_token(p, (int)row, to);
+    part.store(p, row, row_scale(block_max(part.top())), rank, size, ROUTE ? to : targets(p, row), [&](uint2 (&w)[STEPS], int head) {
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) groups[rank + i * size] = w[i];
         if (rank == 0) groups[STEPS * size] = make_uint2(0u, 0u);
@@ -269,7 +329,7 @@ template <typename T, int STEPS, bool ODD> __global__ void __launch_bounds__(256
     if (row >= row_count(p)) return;
     RowPart<T, STEPS, ODD> part;
     part.load(p, row, lane, 32);
-    part.store(p, row, row_scale(__reduce_max_sync(0xffffffffu, part.top())), lane, 32, [&](uint2 (&w)[STEPS], int head) {
+    part.store(p, row, row_scale(__reduce_max_sync(0xffffffffu, part.top())), lane, 32, targets(p, row), [&](uint2 (&w)[STEPS], int head) {
         uint2 behind[STEPS];
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
@@ -293,21 +353,15 @@ template <typename T> __global__ void __launch_bounds__(256) int8_quantize_plain
     uint32_t amax = 0;
     for (int c = threadIdx.x; c < p.k; c += 256) amax = max(amax, __float_as_uint(to_float<T>(x[c])) & 0x7fffffffu);
     const RowScale r = row_scale(block_max(amax));
-    if (threadIdx.x == 0) store_scale(p, row, r.s);
+    const int* to = targets(p, row);
+    if (threadIdx.x == 0) each_target(p, row, to, [&](long long at) { p.scales[at] = r.s; });
     const int kp = (p.k + 15) & ~15;
     for (int c = 4 * threadIdx.x; c < kp; c += 1024) {
         float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = c + j < p.k ? to_float<T>(x[c + j]) : 0.0f;
         const uint32_t w = quantize_any<true>(v[0], v[1], v[2], v[3], r);
-        if (p.position == nullptr) {
-            *reinterpret_cast<uint32_t*>(p.q + row * p.ldq + c) = w;
-        } else {
-            for (int j = 0; j < p.topk; ++j) {
-                const int to = p.position[row * p.topk + j];
-                if (to >= 0) *reinterpret_cast<uint32_t*>(p.q + (long long)to * p.ldq + c) = w;
-            }
-        }
+        each_target(p, row, to, [&](long long at) { *reinterpret_cast<uint32_t*>(p.q + at * p.ldq + c) = w; });
     }
 }
 
@@ -319,23 +373,44 @@ template <typename T, bool ODD> static cudaError_t quantize_held(const QuantizeR
         return launch_kernel(kernel, dim3((unsigned)p.rows, 1, 1), threads, ODD ? (threads * steps + 1) * sizeof(uint2) : 0, s, dependent, p);
     };
     // few rows: every thread as few steps as there can be, the shortest way
-    if (p.rows <= 2 * sms && whole <= 1024) return go(int8_quantize_kernel<T, 1, 1024, ODD>, (unsigned)whole, 1);
+    if (p.rows <= 2 * sms && whole <= 1024) return go(int8_quantize_kernel<T, 1, 1024, ODD, false>, (unsigned)whole, 1);
     if (eights <= 128) {
         const auto kernel = eights <= 32 ? int8_quantize_short_kernel<T, 1, ODD> : (eights <= 64 ? int8_quantize_short_kernel<T, 2, ODD> : int8_quantize_short_kernel<T, 4, ODD>);
         return launch_kernel(kernel, dim3((unsigned)((p.rows + 7) / 8), 1, 1), 256, 0, s, dependent, p);
     }
     const unsigned threads = (unsigned)((eights + 127) / 128 * 32);
-    if (threads <= 512) return go(int8_quantize_kernel<T, 4, 512, ODD>, threads, 4);
-    return go(int8_quantize_kernel<T, 4, 1024, ODD>, threads, 4);
+    if (threads <= 512) return go(int8_quantize_kernel<T, 4, 512, ODD, false>, threads, 4);
+    return go(int8_quantize_kernel<T, 4, 1024, ODD, false>, threads, 4);
 }
+template <typename T> static bool starts_anywhere(const QuantizeRows& p) {
+    return p.k % 8 != 0 || reinterpret_cast<uintptr_t>(p.x) % 16 != 0 || p.ldx * sizeof(T) % 16 != 0;
+}
+template <typename T, bool ODD> static cudaError_t route_held(const QuantizeRows& p, cudaStream_t s) {
+    const unsigned threads = (unsigned)(((p.k + 15) / 16 * 2 + (ODD ? 1 : 0) + 31) / 32 * 32);
+    return launch_kernel(int8_quantize_kernel<T, 1, 1024, ODD, true>, dim3((unsigned)p.rows + 1, 1, 1), threads, ODD ? (threads + 1) * sizeof(uint2) : 0, s, false, p);
+}
+template <typename T> static cudaError_t route_t(const QuantizeRows& p, cudaStream_t s) { return starts_anywhere<T>(p) ? route_held<T, true>(p, s) : route_held<T, false>(p, s); }
+
+// One launch (2 us) less for the layer of experts where every CTA can look at all ids and hold a row.
+bool int8_routes_quantizing(int tokens, int topk, int k) {
+    return topk <= ROUTE_MOST_TOPK && tokens * topk <= ROUTE_MOST_SLOTS && tokens <= 2 * runtime_info().sm_count && k <= 8192 - 16;
+}
+cudaError_t int8_route_quantize(int elem, const void* x, long long ldx, int8_t* q, long long ldq, float* scales, int tokens, int k, const void* ids,
+                                bool wide_ids, int topk, int experts, int* position, int* offsets, cudaStream_t s) {
+    const QuantizeRows p{x, ldx, q, ldq, scales, tokens, k, nullptr, topk, nullptr, ids, wide_ids, experts, position, offsets};
+    if (elem == ELEM_F32) return route_t<float>(p, s);
+    if (elem == ELEM_F16) return route_t<__half>(p, s);
+    return route_t<__nv_bfloat16>(p, s);
+}
+
 template <typename T> static cudaError_t quantize_t(const QuantizeRows& p, cudaStream_t s, bool dependent) {
-    const bool odd = p.k % 8 != 0 || reinterpret_cast<uintptr_t>(p.x) % 16 != 0 || p.ldx * sizeof(T) % 16 != 0;
+    const bool odd = starts_anywhere<T>(p);
     return odd ? quantize_held<T, true>(p, s, dependent) : quantize_held<T, false>(p, s, dependent);
 }
 
 cudaError_t int8_quantize_rows(int elem, const void* x, long long ldx, int8_t* q, long long ldq, float* scales, long long rows, int k,
                                const int* position, int topk, const int* row_limit, cudaStream_t s, bool dependent) {
-    const QuantizeRows p{x, ldx, q, ldq, scales, rows, k, position, topk, row_limit};
+    const QuantizeRows p{x, ldx, q, ldq, scales, rows, k, position, topk, row_limit, nullptr, false, 0, nullptr, nullptr};
     if (elem == ELEM_F32) return quantize_t<float>(p, s, dependent);
     if (elem == ELEM_F16) return quantize_t<__half>(p, s, dependent);
     return quantize_t<__nv_bfloat16>(p, s, dependent);
