@@ -211,11 +211,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
                     const int col = (n >> 4) * 8 + (n & 7), from = is_up ? 16 : 0;
                     const int toks = col < p.n_out ? t.toks - c - from : 0;
                     dst += from * p.ldy + col;
+                    // All sixteen before the first store: under a store's condition the compiler put each value's arithmetic in a branch
+                    // of its own, one after the other (7696 rows of 60 experts, 256 -> 2 x 512 -> 256: 54.3 us the layer, now 44.1).
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
                         const float other = __shfl_xor_sync(0xffffffffu, is_up ? v[j] : v[16 + j], 8);
                         const float gate = is_up ? other : v[j], up = is_up ? v[16 + j] : other;
-                        if (j < toks) *dst = from_float<OutT>(int8_activate(gate, ACT) * up);
+                        v[j] = int8_activate(gate, ACT) * up;
+                        asm volatile("" : "+f"(v[j]));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        if (j < toks) *dst = from_float<OutT>(v[j]);
                         dst += p.ldy;
                     }
                 }
