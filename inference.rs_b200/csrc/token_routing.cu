@@ -14,6 +14,7 @@ namespace b200q {
 constexpr int RT_THREADS = 1024;
 constexpr int RT_HELD = 8;      // ids that a lane reads at once
 constexpr int RT_ROW_THREADS = 256;
+constexpr int RT_ROW_CTAS = 8;  // CTAs of as many threads on an SM
 
 // One CTA per expert, and one more for the slots of none. Each CTA counts by itself how many slots belong to experts before its own
 // (its first row) and ranks its own slots, reading all ids twice: a few hundred KB out of L2 at most, where counting once and ranking
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(RT_ROW_THREADS) route_dispatch_kernel(const U*
     for (int j = 0; j < topk; j += S) {
         int p[S];
         slot_rows(position, t, topk, j, nvalid, p);
-        for (int c = threadIdx.x; c < h; c += blockDim.x) {
+        for (int c = (int)(blockIdx.y * blockDim.x + threadIdx.x); c < h; c += blockDim.x * gridDim.y) {
             const U v = src[c];
 #pragma unroll
             for (int i = 0; i < S; ++i) {
@@ -146,15 +147,21 @@ __global__ void __launch_bounds__(RT_ROW_THREADS) route_dispatch_kernel(const U*
 
 // threads of a CTA that goes over `n` pieces of a row
 static unsigned row_threads(int n) { return n >= RT_ROW_THREADS ? (unsigned)RT_ROW_THREADS : (unsigned)((n + 31) / 32 * 32); }
+// A CTA per token; where the tokens are too few to fill the SMs, more of them, each with its share of the columns (combine, f32, 8 slots,
+// rows of 7168: 16 tokens 6.7 us with one CTA each, 2.6 with seven; 64 tokens 6.9 and 3.3).
+static dim3 row_grid(int tokens, int n, unsigned threads) {
+    const int steps = (n + (int)threads - 1) / (int)threads, room = runtime_info().sm_count * RT_ROW_CTAS / tokens;
+    return dim3((unsigned)tokens, (unsigned)(room < 2 ? 1 : (steps < room ? steps : room)), 1);
+}
 
 cudaError_t route_dispatch(int elem, const void* x, long long ldx, const int* position, const int* valid, void* rows, int tokens, int topk, int h,
                            cudaStream_t s) {
     const int es = elem == ELEM_F32 ? 4 : 2;
-    const dim3 grid((unsigned)tokens, 1, 1);
     const auto go = [&](auto unit, int per) {  // `per` values in a unit
         using U = decltype(unit);
+        const unsigned threads = row_threads(h / per);
         const auto kernel = topk <= 2 ? route_dispatch_kernel<U, 2> : route_dispatch_kernel<U, 4>;
-        return launch_kernel(kernel, grid, row_threads(h / per), 0, s, false, static_cast<const U*>(x), ldx / per, position, valid, static_cast<U*>(rows), topk, h / per);
+        return launch_kernel(kernel, row_grid(tokens, h / per, threads), threads, 0, s, false, static_cast<const U*>(x), ldx / per, position, valid, static_cast<U*>(rows), topk, h / per);
     };
     if (rows_wide(x, ldx, elem) && rows_wide(rows, h, elem)) return go(uint4{}, 16 / es);
     if (es == 4) return go(uint32_t{}, 1);
@@ -179,7 +186,7 @@ __global__ void __launch_bounds__(RT_ROW_THREADS) route_combine_kernel(const In*
         for (int i = 0; i < S; ++i) w[i] = weights == nullptr ? 1.0f : (j + i < topk ? weights[t * topk + j + i] : 0.0f);
     };
     slots(0);
-    for (int c = first_column<V, WIDE>(); c < h; c += V * blockDim.x) {
+    for (int c = first_column<V, WIDE>() + (int)(blockIdx.y * V * blockDim.x); c < h; c += V * blockDim.x * gridDim.y) {
         float sum[V] = {};
         for (int j = 0; j < topk; j += S) {
             if (topk > S) slots(j);
@@ -204,10 +211,11 @@ __global__ void __launch_bounds__(RT_ROW_THREADS) route_combine_kernel(const In*
 template <typename In, typename Out>
 static cudaError_t combine_t(bool wide, const void* rows, long long ldr, const int* position, const float* weights, void* out, int tokens, int topk,
                              int h, cudaStream_t s, bool dependent) {
-    const dim3 grid((unsigned)tokens, 1, 1);
     constexpr int V = 16 / sizeof(Out);
+    const int per = wide ? h / V : (h + 3) / 4;
+    const unsigned threads = row_threads(per);
     const auto kernel = wide ? (topk <= 2 ? route_combine_kernel<In, Out, V, 2, true> : route_combine_kernel<In, Out, V, 4, true>) : route_combine_kernel<In, Out, 4, 4, false>;
-    return launch_kernel(kernel, grid, row_threads(wide ? h / V : (h + 3) / 4), 0, s, dependent, static_cast<const In*>(rows), ldr, position, weights, static_cast<Out*>(out), topk, h);
+    return launch_kernel(kernel, row_grid(tokens, per, threads), threads, 0, s, dependent, static_cast<const In*>(rows), ldr, position, weights, static_cast<Out*>(out), topk, h);
 }
 cudaError_t route_combine(int elem_in, int elem_out, const void* rows, long long ldr, const int* position, const float* weights, void* out,
                           int tokens, int topk, int h, cudaStream_t s, bool dependent) {

@@ -24,7 +24,8 @@ def call_path(request, monkeypatch):
     """Both call paths of the torch front end."""
     if request.param == "python":
         monkeypatch.setattr(kl, "_host", kl.NoNativePath())
-SHAPES = [(1, 1, 1, 1), (1, 8, 2, 64), (7, 128, 8, 100), (33, 60, 4, 1037), (300, 2, 1, 512), (513, 1024, 3, 24), (1000, 5, 6, 130), (64, 16, 16, 2048)]
+SHAPES = [(1, 1, 1, 1), (1, 8, 2, 64), (7, 128, 8, 100), (33, 60, 4, 1037), (300, 2, 1, 512), (513, 1024, 3, 24), (1000, 5, 6, 130), (64, 16, 16, 2048),
+          (3, 4, 2, 5637), (16, 5, 3, 7168), (130, 6, 2, 2100)]  # the last three: several CTAs to a row
 
 
 def choose(tokens, experts, topk, dropped, dtype=torch.int64, seed=0):
