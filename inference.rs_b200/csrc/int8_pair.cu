@@ -24,10 +24,23 @@ struct Int8PairParams {
 struct Int8PairBarriers {
     uint64_t full[I8P_MAX_STAGES], empty[I8P_MAX_STAGES];
     uint64_t tmem_full[2], tmem_empty[2];
-    uint32_t tmem_base;
+    uint32_t tmem_base, unused[3];
+    float xs[I8P_EPILOGUE][I8P_TOKENS / (I8P_EPILOGUE / 4)];  // an epilogue warp's token scales of its tile
 };
 static size_t i8p_smem(int stages, int bn, int experts) {
     return 1024 + (size_t)stages * I8P_SUB * (I8P_A_BYTES + bn / 2 * I8P_BK) + sizeof(Int8PairBarriers) + int8_list_bytes(experts);
+}
+
+// The first `count` of N values, to consecutive rows. (By whole warps.)
+template <int N, typename OutT> __device__ __forceinline__ void store_column(OutT* dst, long long ld, const float* v, int count) {
+    if (__all_sync(0xffffffffu, count >= N)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) dst[j * ld] = from_float<OutT>(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            if (j < count) dst[j * ld] = from_float<OutT>(v[j]);
+    }
 }
 
 template <typename OutT, int ACT>  // ACT: INT8_ACT_NONE, or the activation of a gated product
@@ -171,46 +184,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
         }
     } else if (warp >= 4) {
         // ---------------- epilogue: thread = weight row, 32 tokens at a time; a warp's store is 32 neighbouring outputs ----------------
+        // A tile's scales are asked for when the one before is done, ahead of the wait for the product; those of the tokens go through
+        // shared memory, four to a load, where a shuffle brought one. us, 8192 x 8192 bf16 outputs of 128 k / 2048 k: scales by shuffles and
+        // after the wait 48.0 / 88.5, so 41.8 / 88.9; asked for while the tile before is at work 37.5 / 90.4, with 16 epilogue warps
+        // 38.6 / 90.6, with the accumulator's next columns on their way as well 43.3 / 90.1, bf16 outputs gathered to 16 bytes in shared
+        // memory 51.4 / 90.9.
+        constexpr int STEP = 8 * I8P_EPILOGUE, CHUNKS = I8P_TOKENS / STEP;  // of a warp's 32 tokens, in a tile
         const int quarter = warp & 3, turn = (warp - 4) >> 2;
         grid_dependency_wait();
-        bool ok = true;
+        float* scales = bars->xs[warp - 4];
+        Int8Tile t{};
+        float ws = 0.0f, xs[CHUNKS];
+        const auto ask = [&](int tile) {
+            if (tile >= ntiles) return;
+            t = list.find(tile, lane);
+            const int n = t.tn * 2 * I8P_ROWS + (int)rank * I8P_ROWS + quarter * 32 + lane;
+            ws = n < p.n ? p.ws[(long long)t.e * p.n + n] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < CHUNKS; ++i) {
+                const int c = 32 * turn + i * STEP + lane;
+                xs[i] = c < t.toks ? p.xs[t.row0 + c] : 0.0f;
+            }
+        };
+        ask(pair);
         int ti = 0;
         for (int tile = pair; tile < ntiles; tile += npairs, ++ti) {
-            const int buf = ti & 1;
-            const Int8Tile t = list.find(tile, lane);
-            const int n = t.tn * 2 * I8P_ROWS + (int)rank * I8P_ROWS + quarter * 32 + lane;
-            const float ws = n < p.n ? p.ws[(long long)t.e * p.n + n] : 0.0f;
-            if (!mbar_wait_bounded(&bars->tmem_full[buf], (ti >> 1) & 1)) {
-                record_failure(p.status, STATUS_WAIT_MMA_TIMEOUT, ti);
-                ok = false;
-            }
+            const int buf = ti & 1, toks = t.toks, n = t.tn * 2 * I8P_ROWS + (int)rank * I8P_ROWS + quarter * 32 + lane;
+            const float w = ws;
+            OutT* y = static_cast<OutT*>(p.y) + (long long)t.row0 * p.ldy;
+#pragma unroll
+            for (int i = 0; i < CHUNKS; ++i) scales[32 * i + lane] = xs[i];
+            bool ok = mbar_wait_bounded(&bars->tmem_full[buf], (ti >> 1) & 1);
+            if (!ok) record_failure(p.status, STATUS_WAIT_MMA_TIMEOUT, ti);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc_fence_after();
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + buf * I8P_TOKENS;
-            OutT* y = static_cast<OutT*>(p.y) + (long long)t.row0 * p.ldy;
-            for (int c = 32 * turn; c < t.toks; c += 32 * (I8P_EPILOGUE / 4)) {
-                const float xs = c + lane < t.toks ? p.xs[t.row0 + c + lane] : 0.0f;
-                uint32_t acc[32];
-                tmem_ld_32x32(taddr + c, acc);
+            const auto finish = [&](const uint32_t (&acc)[32], int c) {
                 float v[32];
+                const float* sc = scales + c / STEP * 32;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = (float)(int)acc[j] * __shfl_sync(0xffffffffu, xs, j) * ws;
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(sc + j);
+                    v[j] = (float)(int)acc[j] * x.x * w;
+                    v[j + 1] = (float)(int)acc[j + 1] * x.y * w;
+                    v[j + 2] = (float)(int)acc[j + 2] * x.z * w;
+                    v[j + 3] = (float)(int)acc[j + 3] * x.w * w;
+                }
                 OutT* dst = y + c * p.ldy;
                 if constexpr (ACT == INT8_ACT_NONE) {
-                    dst += n;
-                    const int toks = n < p.n ? t.toks - c : 0;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (j < toks) *dst = from_float<OutT>(v[j]);
-                        dst += p.ldy;
-                    }
+                    store_column<32>(dst + n, p.ldy, v, n < p.n ? toks - c : 0);
                 } else {
                     // rows 8.. of 16 hold up, the others gate: the lane of a gate row takes tokens 0..15, that of its up row 16..31
                     const bool is_up = (lane & 8) != 0;
                     const int col = (n >> 4) * 8 + (n & 7), from = is_up ? 16 : 0;
-                    const int toks = col < p.n_out ? t.toks - c - from : 0;
-                    dst += from * p.ldy + col;
                     // All sixteen before the first store: under a store's condition the compiler put each value's arithmetic in a branch
                     // of its own, one after the other (7696 rows of 60 experts, 256 -> 2 x 512 -> 256: 54.3 us the layer, now 44.1).
 #pragma unroll
@@ -220,13 +247,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
                         v[j] = int8_activate(gate, ACT) * up;
                         asm volatile("" : "+f"(v[j]));
                     }
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        if (j < toks) *dst = from_float<OutT>(v[j]);
-                        dst += p.ldy;
-                    }
+                    store_column<16>(dst + from * p.ldy + col, p.ldy, v, col < p.n_out ? toks - c - from : 0);
                 }
+            };
+            __syncwarp();  // the scales are there
+            for (int c = 32 * turn; c < toks; c += STEP) {
+                uint32_t acc[32];
+                tmem_ld_32x32(taddr + c, acc);
+                finish(acc, c);
             }
+            ask(tile + npairs);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_rank(&bars->tmem_empty[buf], 0));  // the accumulator may be reused
