@@ -69,10 +69,12 @@ __device__ __noinline__ uint32_t quantize_four_carefully(float a, float b, float
 }
 // The remainder settles every value without a branch: one bf16 value in some hundred has a quotient within a rounding of s of a half (127
 // times one 8-bit mantissa by another), so a way out of line for them was taken by every other warp and cost as much as all the rest.
-// HALVES: a value can lie on a half exactly without s being a power of two, for which the rounding of x * (1 / s) is right as it is. Not
-// so for bf16: half an odd multiple of s has 8 bits only where s has one.
+// A value can lie on a half exactly without s being a power of two, for which the rounding of x * (1 / s) is right as it is. Not so for
+// bf16: half an odd multiple of s has 8 bits only where s has one. In an f16 row in a hundred s has few bits and many values lie there: they
+// are settled in line (512 rows of 4096: by a way out of line 5.8 us, now 3.6). f32 values hardly ever do, and the way out of line is the
+// faster one (8192 rows of 14336: 101 us, in line 108.6).
 // Rows of the smallest floats (r.pre) are not for this one.
-template <bool HALVES> __device__ __forceinline__ uint32_t quantize_four(float a, float b, float c, float d, const RowScale& r) {
+template <typename T> __device__ __forceinline__ uint32_t quantize_four(float a, float b, float c, float d, const RowScale& r) {
     const float v[4] = {a, b, c, d};
     float t[4];
     bool on_half = false;
@@ -80,17 +82,20 @@ template <bool HALVES> __device__ __forceinline__ uint32_t quantize_four(float a
     for (int i = 0; i < 4; ++i) {
         t[i] = fmaf(v[i], r.inv, ROUND);
         const float rem = fmaf(ROUND - t[i], r.sn, v[i]);
-        if constexpr (HALVES) on_half |= fabsf(rem) == r.half;
+        if constexpr (sizeof(T) == 4) on_half |= fabsf(rem) == r.half;
         const float step = __uint_as_float((__float_as_uint(rem) & 0x80000000u) | 0x3f800000u);
-        t[i] = fabsf(rem) > r.half ? t[i] + step : t[i];
+        uint32_t size = __float_as_uint(rem) & 0x7fffffffu;
+        // an odd integer gives way to the even one next to it, as if its remainder were larger by the last place
+        if constexpr (std::is_same<T, __half>::value) size += __float_as_uint(t[i]) & 1u;
+        t[i] = __uint_as_float(size) > r.half ? t[i] + step : t[i];
     }
-    if (HALVES && on_half) return quantize_four_carefully(a, b, c, d, r.sn, r.inv, 1.0f);
+    if (sizeof(T) == 4 && on_half) return quantize_four_carefully(a, b, c, d, r.sn, r.inv, 1.0f);
     return __byte_perm(__byte_perm(__float_as_uint(t[0]), __float_as_uint(t[1]), 0x0040), __byte_perm(__float_as_uint(t[2]), __float_as_uint(t[3]), 0x0040), 0x5410);
 }
 
-template <bool HALVES> __device__ __forceinline__ uint32_t quantize_any(float a, float b, float c, float d, const RowScale& r) {
+template <typename T> __device__ __forceinline__ uint32_t quantize_any(float a, float b, float c, float d, const RowScale& r) {
     if (r.inv == 0.0f) return 0u;
-    return r.pre == 1.0f ? quantize_four<HALVES>(a, b, c, d, r) : quantize_four_carefully(a, b, c, d, r.sn, r.inv, r.pre);
+    return r.pre == 1.0f ? quantize_four<T>(a, b, c, d, r) : quantize_four_carefully(a, b, c, d, r.sn, r.inv, r.pre);
 }
 
 // Eight values of a row as they lie in memory. Plain loads: what they read may be the work of the launch before, which this one waited
@@ -116,7 +121,6 @@ template <> struct Eight<float> {
         return max(m, max(max(abs_bits(b.x), abs_bits(b.y)), max(abs_bits(b.z), abs_bits(b.w))));
     }
     static __device__ uint32_t float_bits(uint32_t top) { return top; }
-    static constexpr bool HALVES = true;
     __device__ void get(float (&v)[8]) const {
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
         v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -143,7 +147,6 @@ template <typename T> struct Eight {
         const unsigned short lo = (unsigned short)top, hi = (unsigned short)(top >> 16);
         return max(__float_as_uint(to_float<T>(*reinterpret_cast<const T*>(&lo))) & 0x7fffffffu, __float_as_uint(to_float<T>(*reinterpret_cast<const T*>(&hi))) & 0x7fffffffu);
     }
-    static constexpr bool HALVES = sizeof(T) == 2 && !std::is_same<T, __nv_bfloat16>::value;
     __device__ void get(float (&v)[8]) const {
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
             const uint32_t w[4] = {a.x, a.y, a.z, a.w};
@@ -218,7 +221,7 @@ template <typename T, int STEPS, bool ODD> struct RowPart {
         for (int i = 0; i < STEPS; ++i) {
             float v[8];
             held[i].get(v);
-            w[i] = make_uint2(quantize_any<Eight<T>::HALVES>(v[0], v[1], v[2], v[3], r), quantize_any<Eight<T>::HALVES>(v[4], v[5], v[6], v[7], r));
+            w[i] = make_uint2(quantize_any<T>(v[0], v[1], v[2], v[3], r), quantize_any<T>(v[4], v[5], v[6], v[7], r));
         }
         if constexpr (ODD) next(w, head);
 #pragma unroll
@@ -320,7 +323,10 @@ template <typename T, int STEPS, int MAX_THREADS, bool ODD, bool ROUTE> __global
         for (int i = 0; i < STEPS; ++i) w[i] = shifted(w[i], groups[rank + i * size + 1], head);
     });
 }
-// A warp per row, rows of up to 1024 values: a CTA for each such row would cost its start, about a nanosecond.
+// A warp per row, rows of up to 1024 values, of up to 1536 where there are many: a CTA for each such row would cost its start, about a
+// nanosecond (bf16 of 1408: 24576 rows 28.9 us by CTAs, 21.5 by warps; 1024 rows 3.3 and 3.1, 512 2.9 and 3.1; of 2048, 24576 rows, 29.3
+// and 27.1, f32 38.8 and 39.6).
+constexpr int SHORT_ROWS = 1024;
 template <typename T, int STEPS, bool ODD> __global__ void __launch_bounds__(256) int8_quantize_short_kernel(const QuantizeRows p) {
     grid_dependency_wait();
     grid_launch_dependents();
@@ -360,7 +366,7 @@ template <typename T> __global__ void __launch_bounds__(256) int8_quantize_plain
         float v[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[j] = c + j < p.k ? to_float<T>(x[c + j]) : 0.0f;
-        const uint32_t w = quantize_any<true>(v[0], v[1], v[2], v[3], r);
+        const uint32_t w = quantize_any<T>(v[0], v[1], v[2], v[3], r);
         each_target(p, row, to, [&](long long at) { *reinterpret_cast<uint32_t*>(p.q + at * p.ldq + c) = w; });
     }
 }
@@ -374,8 +380,9 @@ template <typename T, bool ODD> static cudaError_t quantize_held(const QuantizeR
     };
     // few rows: every thread as few steps as there can be, the shortest way
     if (p.rows <= 2 * sms && whole <= 1024) return go(int8_quantize_kernel<T, 1, 1024, ODD, false>, (unsigned)whole, 1);
-    if (eights <= 128) {
-        const auto kernel = eights <= 32 ? int8_quantize_short_kernel<T, 1, ODD> : (eights <= 64 ? int8_quantize_short_kernel<T, 2, ODD> : int8_quantize_short_kernel<T, 4, ODD>);
+    if (eights <= 128 || (eights <= 192 && p.rows >= SHORT_ROWS)) {
+        const auto kernel = eights <= 32 ? int8_quantize_short_kernel<T, 1, ODD> : eights <= 64 ? int8_quantize_short_kernel<T, 2, ODD>
+                          : eights <= 128 ? int8_quantize_short_kernel<T, 4, ODD> : int8_quantize_short_kernel<T, 6, ODD>;
         return launch_kernel(kernel, dim3((unsigned)((p.rows + 7) / 8), 1, 1), 256, 0, s, dependent, p);
     }
     const unsigned threads = (unsigned)((eights + 127) / 128 * 32);

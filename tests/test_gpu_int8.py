@@ -96,6 +96,34 @@ def test_rows_of_the_smallest_numbers(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_quotients_on_a_half(dtype):
+    """Scales of few bits, m 2^e, have values whose quotients are halves exactly: all that the type holds, among their neighbours."""
+    rows = []
+    for m in range(1, 17):
+        for e in (-12, -5, 0, 4):
+            s = m * 2.0 ** e
+            half = ((torch.arange(-127, 127).double() + 0.5) * s).to(dtype)
+            inf = torch.tensor(math.inf, dtype=dtype)
+            row = torch.cat([half, torch.nextafter(half, inf), torch.nextafter(half, -inf)]).clamp(-127 * s, 127 * s)
+            row[0] = 127 * s
+            rows.append(row)
+    x = torch.stack(rows).cuda()
+    for x in (x, x.repeat(20, 2)):
+        want_q, want_s = rows64(x)
+        q, s = ops.int8_quantize(x)
+        assert torch.equal(s, want_s) and torch.equal(q[:, :x.shape[1]].double(), want_q)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("k", [1025, 1032, 1408, 1409, 1529, 1536, 1537, 1544])
+def test_quantize_of_many_rows_of_middling_length(k, dtype):
+    x = acts(1100, k + 3, dtype)[:, 3 * (k % 2):][:, :k]
+    want_q, want_s = rows64(x)
+    q, s = ops.int8_quantize(x)
+    assert torch.equal(q[:, :k].double(), want_q) and torch.equal(s, want_s) and not q[:, k:].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_quantize_of_strided_and_unaligned_rows(dtype):
     big, wide, many = acts(9, 300, dtype), acts(6, 9000, dtype), acts(700, 1100, dtype)
     parts = [big[:, i:i + n] for i in range(9) for n in (1, 7, 8, 9, 15, 16, 17, 250)]
