@@ -68,19 +68,23 @@ inline constexpr size_t int8_list_bytes(int experts) { return experts > 1 ? 8 * 
 struct Int8TileList {
     const int* start;    // shared memory: tiles before each expert's, experts + 1 of them (null: one matrix)
     const int* offsets;  // shared memory
-    int experts, rows, bn, tiles_n, ntiles, at;
+    int experts, row0, rows, bn, tiles_n, ntiles, at;
 
     // by all threads of a CTA; `shared`: int8_list_bytes
     template <int THREADS> __device__ __forceinline__ void build(const Int8Product& p, int bn_, int tiles_n_, int* shared) {
         start = offsets = nullptr;
         experts = p.experts;
+        row0 = 0;
         rows = p.rows;
         bn = bn_;
         tiles_n = tiles_n_;
         at = 0;
         if (p.offsets != nullptr) grid_dependency_wait();  // where the experts' rows begin is the work of a launch before
         if (experts == 1) {
-            if (p.offsets != nullptr) rows = min(max(p.offsets[1], 0), p.rows);
+            if (p.offsets != nullptr) {
+                row0 = min(max(p.offsets[0], 0), p.rows);
+                rows = max(min(p.offsets[1], p.rows) - row0, 0);
+            }
             ntiles = (rows + bn - 1) / bn * tiles_n;
             return;
         }
@@ -114,7 +118,7 @@ struct Int8TileList {
     // by whole warps, with tiles that do not fall
     __device__ __forceinline__ Int8Tile find(int tile, int lane) {
         Int8Tile t;
-        int first = 0, count = rows;
+        int first = row0, count = rows;
         t.e = 0;
         if (start != nullptr) {
             for (;; at += 32) {

@@ -310,6 +310,21 @@ def test_rows_meet_their_experts_matrix(counts, n, k):
     assert_device_ok()
 
 
+@pytest.mark.parametrize("rows,n,k", [(9, 40, 100), (60, 520, 1024), (700, 300, 512)])
+@pytest.mark.parametrize("experts", [1, 2])
+def test_rows_before_the_first_offset_belong_to_none(experts, rows, n, k):
+    w, x = int8_weight(experts, n, k), acts(rows, k, torch.float32)
+    xq, xs = ops.int8_quantize(x)
+    for first, last in ((4, rows - 2), (rows - 1, rows), (3, 3), (5, 2), (rows + 5, rows + 9)):
+        offsets = torch.tensor([first, *[last] * experts], dtype=torch.int32, device="cuda")
+        out = torch.full((rows, n), 7.0, device="cuda")
+        ops.int8_gemm(xq, xs, w.data, w.scales, k, torch.float32, offsets, out)
+        want = (xq[:, :k].double() @ w.data[0, :, :k].double().T) * xs.double()[:, None] * w.scales[0].double()
+        close(out[first:last], want[first:last])
+        assert (out[:first] == 7).all() and (out[max(first, last):] == 7).all()
+    assert_device_ok()
+
+
 def check_experts(counts, n, k, dtype):
     w, x = int8_weight(len(counts), n, k), acts(sum(counts), k, torch.float32)
     xq, xs = ops.int8_quantize(x)
