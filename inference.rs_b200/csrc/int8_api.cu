@@ -20,6 +20,8 @@ static int check_k(int k) {
     if (k > INT8_MAX_K) return set_error(B200Q_ERR_UNSUPPORTED, "sums of more than 131071 int8 products do not fit 32 bits");
     return B200Q_OK;
 }
+// a step over a row's columns is less than 2^20 of them
+static bool columns_ok(int h) { return h >= 0 && h <= INT_MAX - (1 << 20); }
 static int check_routing(long long tokens, int topk, int experts) {
     if (tokens < 0 || topk < 1) return set_error(B200Q_ERR_INVALID, "a negative number of tokens, or no slots");
     if (experts < 1 || experts > INT8_MAX_EXPERTS) return set_error(B200Q_ERR_UNSUPPORTED, "1 to 1024 experts");
@@ -146,7 +148,7 @@ int b200q_route_dispatch(int elem, const void* x, long long ldx, const int* posi
                          int topk, int h, void* stream) {
     if (!elem_ok(elem)) return set_error(B200Q_ERR_UNSUPPORTED, "rows are f32, f16 or bf16");
     if (const int rc = check_routing(tokens, topk, experts)) return rc;
-    if (h < 0 || ldx < h) return set_error(B200Q_ERR_INVALID, "bad shape");
+    if (!columns_ok(h) || ldx < h) return set_error(B200Q_ERR_INVALID, "bad shape");
     if (tokens == 0 || h == 0) return B200Q_OK;
     if (!x || !position || !offsets || !rows) return set_error(B200Q_ERR_INVALID, "null pointer");
     return cuda_result(route_dispatch(elem, x, ldx, position, offsets + experts, rows, tokens, topk, h, (cudaStream_t)stream));
@@ -156,7 +158,7 @@ int b200q_route_combine(int elem_in, int elem_out, const void* rows, long long l
                         int topk, int h, void* stream) {
     if (!elem_ok(elem_in) || !elem_ok(elem_out)) return set_error(B200Q_ERR_UNSUPPORTED, "rows are f32, f16 or bf16");
     if (const int rc = check_routing(tokens, topk, 1)) return rc;
-    if (h < 0 || ldr < h) return set_error(B200Q_ERR_INVALID, "bad shape");
+    if (!columns_ok(h) || ldr < h) return set_error(B200Q_ERR_INVALID, "bad shape");
     if (tokens == 0 || h == 0) return B200Q_OK;
     if (!rows || !position || !out) return set_error(B200Q_ERR_INVALID, "null pointer");
     return cuda_result(route_combine(elem_in, elem_out, rows, ldr, position, weights, out, tokens, topk, h, (cudaStream_t)stream, false));
@@ -167,7 +169,7 @@ int b200q_route_combine_grad(int elem_grad, int elem, const void* grad_out, long
                              int h, void* stream) {
     if (!elem_ok(elem_grad) || !elem_ok(elem)) return set_error(B200Q_ERR_UNSUPPORTED, "rows are f32, f16 or bf16");
     if (const int rc = check_routing(tokens, topk, experts)) return rc;
-    if (h < 0 || ldg < h || (grad_weights && ldr < h)) return set_error(B200Q_ERR_INVALID, "bad shape");
+    if (!columns_ok(h) || ldg < h || (grad_weights && ldr < h)) return set_error(B200Q_ERR_INVALID, "bad shape");
     if (tokens == 0 || (!grad_rows && !grad_weights)) return B200Q_OK;
     if (!position || !offsets || !weights || (h > 0 && (!grad_out || (grad_weights && !rows)))) return set_error(B200Q_ERR_INVALID, "null pointer");
     return cuda_result(route_combine_grad(elem_grad, elem, grad_out, ldg, rows, ldr, position, offsets + experts, weights, grad_rows, grad_weights, tokens, topk, h, (cudaStream_t)stream));

@@ -150,7 +150,7 @@ static unsigned row_threads(int n) { return n >= RT_ROW_THREADS ? (unsigned)RT_R
 // A CTA per token; where the tokens are too few to fill the SMs, more of them, each with its share of the columns (combine, f32, 8 slots,
 // rows of 7168: 16 tokens 6.7 us with one CTA each, 2.6 with seven; 64 tokens 6.9 and 3.3).
 static dim3 row_grid(int tokens, int n, unsigned threads) {
-    const int steps = (n + (int)threads - 1) / (int)threads, room = runtime_info().sm_count * RT_ROW_CTAS / tokens;
+    const int steps = min((n + (int)threads - 1) / (int)threads, 256), room = runtime_info().sm_count * RT_ROW_CTAS / tokens;
     return dim3((unsigned)tokens, (unsigned)(room < 2 ? 1 : (steps < room ? steps : room)), 1);
 }
 

@@ -94,3 +94,7 @@ def test_the_library_refuses_what_it_cannot_take():
     assert lib.b200q_int8_experts(2, 0, 16, 16, 16, 4, 16, 16, 16, 16, 16, 16, 1, 4, 2, 16, 16, 256, 16, None) == -4
     assert lib.b200q_int8_matmul_workspace_bytes(3, 37) >= 3 * 48 + 12
     assert lib.b200q_int8_experts_workspace_bytes(2, 0, 2, 4, 16, 16) == 0
+    most = 2 ** 31 - 1  # columns: a kernel's step over them would pass 32 bits
+    assert lib.b200q_route_dispatch(0, 16, most, 16, 16, 4, 16, 1, 2, most, None) == -2
+    assert lib.b200q_route_combine(0, 0, 16, most, 16, 16, 16, 1, 2, most, None) == -2
+    assert lib.b200q_route_combine_grad(0, 0, 16, most, 16, most, 16, 16, 4, 16, 16, 16, 1, 2, most, None) == -2
