@@ -22,7 +22,7 @@ def _no_grad_through(*tensors: torch.Tensor) -> None:
 
 class Int8Tensor:
     """int8 rows with a scale each: a matrix [n, k], or one for each expert [experts, n, k]. `data` holds the rows padded to 16 bytes
-    with zeros, `scales` [n] or [experts, n] their scales; row i stands for data[i] * scales[i]."""
+    with zeros, `scales` [n] or [experts, n] their scales, constants to autograd; row i stands for data[i] * scales[i]."""
 
     def __init__(self, data: torch.Tensor, scales: torch.Tensor):
         if data.dtype != torch.int8 or scales.dtype != torch.float32:
@@ -37,7 +37,7 @@ class Int8Tensor:
             padded = data.new_zeros(*data.shape[:-1], kp)
             padded[..., :k] = data
             data = padded
-        self.data, self.scales = data, scales.contiguous()
+        self.data, self.scales = data, scales.detach().contiguous()
 
     @classmethod
     def _of_rows(cls, q: torch.Tensor, scales: torch.Tensor, shape: tuple[int, ...]) -> "Int8Tensor":

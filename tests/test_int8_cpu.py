@@ -98,3 +98,8 @@ def test_the_library_refuses_what_it_cannot_take():
     assert lib.b200q_route_dispatch(0, 16, most, 16, 16, 4, 16, 1, 2, most, None) == -2
     assert lib.b200q_route_combine(0, 0, 16, most, 16, 16, 16, 1, 2, most, None) == -2
     assert lib.b200q_route_combine_grad(0, 0, 16, most, 16, most, 16, 16, 4, 16, 16, 16, 1, 2, most, None) == -2
+
+
+def test_scales_are_constants():
+    scales = torch.rand(4, requires_grad=True)
+    assert not pkg.Int8Tensor(torch.zeros(4, 16, dtype=torch.int8), scales).scales.requires_grad
