@@ -57,6 +57,10 @@ struct Int8Product {
     int n_out;         // columns of y: n, or, gated, the pairs that are real
     long long ldy;
     unsigned int* status;
+    // offsets are older than the launch before this one, which lets this one begin only when it has waited for all before it: they are
+    // read (out of L2) and the first weights asked for without a wait (experts' layer, 1 token through 2 of 8 experts of 4096 x 14336
+    // 67.8 -> 66.2 us, 1024 through 8 of 128 of 2048 x 768 157.3 -> 152.0)
+    bool offsets_known;
 };
 
 // Where a tile of a product lies: its weight tile, its expert, its tokens.
@@ -79,18 +83,18 @@ struct Int8TileList {
         bn = bn_;
         tiles_n = tiles_n_;
         at = 0;
-        if (p.offsets != nullptr) grid_dependency_wait();  // where the experts' rows begin is the work of a launch before
+        if (p.offsets != nullptr && !p.offsets_known) grid_dependency_wait();  // where the experts' rows begin is the work of a launch before
         if (experts == 1) {
             if (p.offsets != nullptr) {
-                row0 = min(max(p.offsets[0], 0), p.rows);
-                rows = max(min(p.offsets[1], p.rows) - row0, 0);
+                row0 = min(max(__ldcg(p.offsets), 0), p.rows);
+                rows = max(min(__ldcg(p.offsets + 1), p.rows) - row0, 0);
             }
             ntiles = (rows + bn - 1) / bn * tiles_n;
             return;
         }
         const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
         int *scan = shared, *off = shared + 32, *st = off + experts + 1;
-        for (int i = tid; i <= experts; i += THREADS) off[i] = min(max(p.offsets[i], 0), p.rows);
+        for (int i = tid; i <= experts; i += THREADS) off[i] = min(max(__ldcg(p.offsets + i), 0), p.rows);
         __syncthreads();
         const int per = (experts + THREADS - 1) / THREADS, e0 = tid * per, e1 = min(e0 + per, experts);
         int sum = 0;

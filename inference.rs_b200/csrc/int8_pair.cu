@@ -90,7 +90,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8P_THREADS, 1)
         const uint32_t full0 = map_to_rank(&bars->full[0], 0);
         // The weights are no launch's work: the first stages' are on their way before the rows are there.
         int early = 0;
-        if (p.offsets == nullptr && pair < ntiles) {
+        if ((p.offsets == nullptr || p.offsets_known) && pair < ntiles) {
             const Int8Tile t = list.find(pair, lane);
             const int row = t.e * p.n + t.tn * 2 * I8P_ROWS + (int)rank * I8P_ROWS;
             early = min(stages, nst);

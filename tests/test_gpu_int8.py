@@ -457,6 +457,23 @@ def test_experts(tokens, experts, topk, hidden, ffn, dropped, dtype):
     assert_device_ok()
 
 
+@pytest.mark.parametrize("tokens,experts,topk", [(1, 8, 2), (40, 16, 4), (300, 16, 2), (1500, 3, 2)])
+def test_layers_one_after_the_other_see_their_own_routing(tokens, experts, topk):
+    """Calls follow each other in the same memory, their launches overlapping: none may see what the call before left."""
+    layer = pkg.Int8Experts(*(int8_weight(experts, *s, seed=i) for i, s in enumerate([(352, 512), (352, 512), (512, 352)])))
+    x = acts(tokens, 512, torch.bfloat16)
+    routes = [router(tokens, experts, topk, dropped, seed) for seed, dropped in ((1, 0.0), (2, 0.5), (3, 1.0), (4, 0.0))]
+    want = []
+    for ids, weights in routes:
+        want.append(layer(x, ids, weights).clone())
+        torch.cuda.synchronize()
+    off = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(200):
+        off += (layer(x, *routes[i % 4]) != want[i % 4]).sum()
+    assert off.item() == 0 and (want[2] == 0).all()
+    assert_device_ok()
+
+
 def test_experts_are_the_operators_one_after_the_other():
     """Routing, rows, products and combination, called one by one, give the layer's bits (ReLU: nothing of its arithmetic differs
     between this library and torch)."""
