@@ -61,7 +61,40 @@ struct Int8Product {
     // read (out of L2) and the first weights asked for without a wait (experts' layer, 1 token through 2 of 8 experts of 4096 x 14336
     // 67.8 -> 66.2 us, 1024 through 8 of 128 of 2048 x 768 157.3 -> 152.0)
     bool offsets_known;
+    const void* ids;  // the slots' expert ids, from which a CTA finds the offsets by itself, known as they are (null: it reads them)
+    bool wide_ids;
 };
+
+__device__ __forceinline__ int expert_id(const void* ids, bool wide, int experts, int slot) {  // `experts`: of none
+    const long long id = wide ? static_cast<const long long*>(ids)[slot] : static_cast<const int*>(ids)[slot];
+    return id >= 0 && id < experts ? (int)id : experts;
+}
+// Where the experts' rows begin, from the slots' ids, by all threads of a CTA: off[0 .. experts] in shared memory. (Out of line: in line, its
+// instructions cost the products that do not call it 0.6 us.)
+static __device__ __noinline__ void expert_offsets(const void* ids, bool wide, int experts, int slots, int* off) {
+    for (int e = threadIdx.x; e <= experts; e += blockDim.x) off[e] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < slots; i += blockDim.x) {
+        const int e = expert_id(ids, wide, experts, i);
+        if (e < experts) atomicAdd(&off[e], 1);  // (integers: any order)
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int sum = 0;
+        for (int e0 = 0; e0 <= experts; e0 += 32) {
+            const int e = e0 + threadIdx.x, c = e < experts ? off[e] : 0;
+            int upto = c;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, d);
+                if ((int)threadIdx.x >= d) upto += v;
+            }
+            if (e <= experts) off[e] = sum + upto - c;
+            sum += __shfl_sync(0xffffffffu, upto, 31);
+        }
+    }
+    __syncthreads();
+}
 
 // Where a tile of a product lies: its weight tile, its expert, its tokens.
 struct Int8Tile {
@@ -94,8 +127,12 @@ struct Int8TileList {
         }
         const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
         int *scan = shared, *off = shared + 32, *st = off + experts + 1;
-        for (int i = tid; i <= experts; i += THREADS) off[i] = min(max(__ldcg(p.offsets + i), 0), p.rows);
-        __syncthreads();
+        if (p.ids != nullptr) {
+            expert_offsets(p.ids, p.wide_ids, experts, p.rows, off);
+        } else {
+            for (int i = tid; i <= experts; i += THREADS) off[i] = min(max(__ldcg(p.offsets + i), 0), p.rows);
+            __syncthreads();
+        }
         const int per = (experts + THREADS - 1) / THREADS, e0 = tid * per, e1 = min(e0 + per, experts);
         int sum = 0;
         for (int e = e0; e < e1; ++e) sum += (max(off[e + 1] - off[e], 0) + bn - 1) / bn * tiles_n;

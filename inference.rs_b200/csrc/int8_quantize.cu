@@ -245,10 +245,7 @@ __device__ __forceinline__ long long row_count(const QuantizeRows& p) {
 // Routing for few slots, without a launch of its own: the CTA of a token counts through all ids where its own slots go, and one more CTA
 // finds where the experts' rows begin. What route_sort_kernel would give, in the same order.
 constexpr int ROUTE_MOST_SLOTS = 2048, ROUTE_MOST_TOPK = 8;
-__device__ __forceinline__ int expert_id(const QuantizeRows& p, int slot) {  // `experts`: of none
-    const long long id = p.wide_ids ? static_cast<const long long*>(p.ids)[slot] : static_cast<const int*>(p.ids)[slot];
-    return id >= 0 && id < p.experts ? (int)id : p.experts;
-}
+__device__ __forceinline__ int expert_id(const QuantizeRows& p, int slot) { return expert_id(p.ids, p.wide_ids, p.experts, slot); }
 __device__ __forceinline__ void route_token(const QuantizeRows& p, int token, int (&to)[ROUTE_MOST_TOPK]) {
     const int slots = (int)p.rows * p.topk, first = token * p.topk;
     int mine[ROUTE_MOST_TOPK], before[ROUTE_MOST_TOPK] = {};
@@ -274,26 +271,6 @@ __device__ __forceinline__ void route_token(const QuantizeRows& p, int token, in
     }
     __syncthreads();
 }
-__device__ __forceinline__ void route_offsets(const QuantizeRows& p, int (&count)[INT8_MAX_EXPERTS + 1]) {
-    for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) count[e] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < (int)p.rows * p.topk; i += blockDim.x) atomicAdd(&count[expert_id(p, i)], 1);
-    __syncthreads();
-    if (threadIdx.x >= 32) return;
-    int sum = 0;
-    for (int e0 = 0; e0 <= p.experts; e0 += 32) {
-        const int e = e0 + threadIdx.x, c = e < p.experts ? count[e] : 0;
-        int upto = c;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, d);
-            if ((int)threadIdx.x >= d) upto += v;
-        }
-        if (e <= p.experts) p.offsets[e] = sum + upto - c;
-        sum += __shfl_sync(0xffffffffu, upto, 31);
-    }
-}
-
 // A CTA per row; ODD rows pass their integers on through shared memory. ROUTE: see above.
 template <typename T, int STEPS, int MAX_THREADS, bool ODD, bool ROUTE> __global__ void __launch_bounds__(MAX_THREADS) int8_quantize_kernel(const QuantizeRows p) {
     extern __shared__ uint2 groups[];
@@ -302,9 +279,10 @@ template <typename T, int STEPS, int MAX_THREADS, bool ODD, bool ROUTE> __global
     grid_launch_dependents();
     const long long row = blockIdx.x;
     if constexpr (ROUTE) {
-        __shared__ int count[INT8_MAX_EXPERTS + 1];
+        __shared__ int off[INT8_MAX_EXPERTS + 1];
         if (row == p.rows) {
-            route_offsets(p, count);
+            expert_offsets(p.ids, p.wide_ids, p.experts, (int)p.rows * p.topk, off);
+            for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) p.offsets[e] = off[e];
             return;
         }
     } else {
