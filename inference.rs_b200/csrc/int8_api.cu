@@ -202,9 +202,9 @@ int b200q_int8_experts(int elem, int activation, const void* x, long long ldx, c
     cudaStream_t s = (cudaStream_t)stream;
     // Where the experts' rows begin is known to the products: the launch before has waited for the one that wrote it, or, where the
     // quantizer does, the product of gate and up counts the ids for itself while there are few, in all and of an expert. us, waiting ->
-    // counting: 1 token through 2 of 8 experts of 4096 x 14336 66.3 -> 65.0, 1 through 8 of 128 of 2048 x 768 20.1 -> 18.5, 54 through 7 of
-    // 64 of 1024 x 512 33.7 -> 31.9, but 190 through 2 of 8 21.2 -> 22.3 and 290 through 7 of 64 44.2 -> 47.2.
-    const bool routes = int8_routes_quantizing(tokens, topk, hidden), counts = routes && experts > 1 && slots <= 384 && slots <= 16 * experts;
+    // counting: 1 token through 2 of 8 experts of 4096 x 14336 66.3 -> 65.0, 1 through 8 of 128 of 2048 x 768 20.1 -> 18.5, 64 through 8 of
+    // 128 100.5 -> 98.2, 128 of them 115.2 -> 114.3, but 256 122.1 -> 125.4, and 190 through 2 of 8 of 1024 x 512 21.4 -> 22.0.
+    const bool routes = int8_routes_quantizing(tokens, topk, hidden), counts = routes && experts > 1 && slots <= 1024 && slots <= 12 * experts;
     const Int8Product up{w.xq, w.xs, static_cast<const int8_t*>(gate_up), gate_up_scales, w.hidden, w.offsets, slots, 2 * pairs, hidden, (int)w.ldx, (int)w.ldx, experts, activation, ffn, w.ldh, status_ptr(), !routes || counts, counts ? ids : nullptr, id_bytes == 8};
     const Int8Product dn{w.hq, w.hs, static_cast<const int8_t*>(down), down_scales, w.y, w.offsets, slots, hidden, ffn, (int)w.ldh, (int)w.ldh, experts, INT8_ACT_NONE, hidden, w.ldy, status_ptr(), true, nullptr, false};
     if (routes) {
