@@ -10,6 +10,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/_to_copy.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -527,6 +528,8 @@ bool row_stride(const Tensor& t, int64_t& ld) {
     return t.size(0) > 1 && t.size(1) > 1 && t.stride(1) == 1 && ld >= t.size(1);
 }
 bool wants_grad(const Tensor& t) { return t.requires_grad() && c10::GradMode::is_enabled(); }
+// a derivative of forward mode, which is there without requires_grad and under no_grad too
+bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode(); }
 // in a backward pass there is no interpreter to raise with
 void require(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed with status ", rc, ": ", abi.last_error()); }
 
@@ -536,7 +539,7 @@ PyObject* py_int8_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     long n, k;
     if (nargs != 5 || !int_args(args, {{2, &n}, {3, &k}})) return none();
     const Tensor *w = tensor_arg(args[0]), *ws = tensor_arg(args[1]), *x = tensor_arg(args[4]);
-    if (!of(w, ScalarType::Char) || !of(ws, ScalarType::Float) || !cuda_contiguous(x) || x->dim() < 2 || x->size(-1) != k || k < 1 || n < 1 || n > MOST || wants_grad(*x)) return none();
+    if (!of(w, ScalarType::Char) || !of(ws, ScalarType::Float) || !cuda_contiguous(x) || x->dim() < 2 || x->size(-1) != k || k < 1 || n < 1 || n > MOST || wants_grad(*x) || has_tangent(*x)) return none();
     const int64_t kp = pad(k, INT8_ROW_ALIGN), m = x->numel() / k;
     const int elem = elem_of(x->scalar_type());
     if (elem < 0 || m == 0 || m > MOST || w->dim() != 2 || w->size(0) != n || w->size(1) != kp || ws->numel() != n || !same_device(*x, {w, ws})) return none();
@@ -601,7 +604,7 @@ PyObject* py_int8_experts(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (elem < 0 || (ids.scalar_type() != ScalarType::Int && ids.scalar_type() != ScalarType::Long) || weights.scalar_type() != ScalarType::Float ||
         gate_up.scalar_type() != ScalarType::Char || down.scalar_type() != ScalarType::Char || gus.scalar_type() != ScalarType::Float || ds.scalar_type() != ScalarType::Float ||
         x.dim() < 2 || ids.dim() != x.dim() || ids.sizes() != weights.sizes() || gate_up.dim() != 3 || down.dim() != 3 || ffn < 1 || x.numel() == 0 || ids.numel() == 0 ||
-        wants_grad(x) || wants_grad(weights) || !same_device(x, {t[1], t[2], t[3], t[4], t[5], t[6]}))
+        wants_grad(x) || wants_grad(weights) || has_tangent(x) || has_tangent(weights) || !same_device(x, {t[1], t[2], t[3], t[4], t[5], t[6]}))
         return none();
     for (int64_t i = 0; i + 1 < x.dim(); ++i)
         if (x.size(i) != ids.size(i)) return none();
@@ -663,6 +666,7 @@ Tensor grad_rows_of(const Tensor& g, int64_t& ld) {
     ld = c.size(1);
     return c;
 }
+void no_tangent(const Tensor& grad) { TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(grad), "the routing of tokens has no derivatives in forward mode, nor do its gradients"); }
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
@@ -676,6 +680,7 @@ struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const Tensor position = ctx->get_saved_variables()[0];
         TORCH_CHECK(!c10::GradMode::is_enabled(), "the gradient of dispatch cannot be differentiated again (create_graph)");
+        no_tangent(grads[0]);
         int64_t ld;
         const Tensor g = grad_rows_of(grads[0], ld);
         return {combine(g, ld, position, nullptr, (ScalarType)ctx->saved_data["type"].toInt()), Tensor(), Tensor()};
@@ -692,6 +697,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &rows = saved[0], &weights = saved[1], &position = saved[2], &offsets = saved[3];
         TORCH_CHECK(!c10::GradMode::is_enabled(), "the gradient of combine cannot be differentiated again (create_graph)");
+        no_tangent(grads[0]);
         int64_t ldg, ldr;
         const Tensor g = grad_rows_of(grads[0], ldg);
         TORCH_CHECK(row_stride(rows, ldr));
@@ -715,7 +721,7 @@ PyObject* py_route_dispatch(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
     const Tensor *x = tensor_arg(args[0]), *position = tensor_arg(args[1]), *offsets = tensor_arg(args[2]);
     int64_t ld;
     if (x == nullptr || !x->is_cuda() || !row_stride(*x, ld) || elem_of(x->scalar_type()) < 0 || x->numel() == 0 || x->size(1) > MOST || !of(position, ScalarType::Int) || position->dim() < 2 ||
-        position->numel() == 0 || position->numel() / position->size(-1) != x->size(0) || !of(offsets, ScalarType::Int) || offsets->numel() < 2 || !same_device(*x, {position, offsets}))
+        position->numel() == 0 || position->numel() / position->size(-1) != x->size(0) || !of(offsets, ScalarType::Int) || offsets->numel() < 2 || !same_device(*x, {position, offsets}) || has_tangent(*x))
         return none();
     Tensor rows;
     {
@@ -736,7 +742,7 @@ PyObject* py_route_combine(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     int64_t ld;
     if (rows == nullptr || !rows->is_cuda() || !row_stride(*rows, ld) || elem_of(rows->scalar_type()) < 0 || rows->numel() == 0 || rows->size(1) > MOST || !of(weights, ScalarType::Float) ||
         !of(position, ScalarType::Int) || position->dim() < 2 || position->sizes() != weights->sizes() || position->numel() != rows->size(0) || !of(offsets, ScalarType::Int) ||
-        offsets->numel() < 2 || !same_device(*rows, {weights, position, offsets}))
+        offsets->numel() < 2 || !same_device(*rows, {weights, position, offsets}) || has_tangent(*rows) || has_tangent(*weights))
         return none();
     Tensor out;
     {

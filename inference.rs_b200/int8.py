@@ -18,6 +18,8 @@ from .qmatmul import QTensor
 def _no_grad_through(*tensors: torch.Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError("int8 products have no gradient: call them under torch.no_grad(), or on detached tensors")
+    if ops.has_tangent(*tensors):
+        raise ValueError("int8 products have no gradient in forward mode either: call them on primals")
 
 
 class Int8Tensor:

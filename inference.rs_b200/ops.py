@@ -11,6 +11,7 @@ import functools
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import kernel_library as kl
 from .dtypes import (ELEM_BF16, ELEM_F16, ELEM_F32, ELEM_TAG, MATRIX_ROW_PADDING, MMQ_TYPE_X, GgmlDType, pad)
@@ -375,6 +376,11 @@ def _one_device(*tensors: torch.Tensor) -> torch.device:
         if t.device != tensors[0].device:
             raise ValueError(f"tensors on {tensors[0].device} and {t.device}")
     return tensors[0].device
+
+
+def has_tangent(*tensors: torch.Tensor) -> bool:
+    """A derivative of forward mode comes with one of them: it is there without `requires_grad`, and under `no_grad` too."""
+    return torch._C._is_fwd_grad_enabled() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _rows2d(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int]:

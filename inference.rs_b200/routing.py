@@ -2,7 +2,8 @@
 
 A router gives every token a few experts (`ids`) and a weight for each. `TokenRouting` sorts the slots by expert once; `dispatch` brings
 the tokens into that order, one row per slot, `combine` adds a token's rows up again with the weights applied. Both can be
-differentiated; their sums run in slot order and in 32 bits, so that results and gradients are the same bits every time.
+differentiated in reverse mode (what carries a tangent of forward mode is refused); their sums run in slot order and in 32 bits, so
+that results and gradients are the same bits every time.
 """
 from __future__ import annotations
 
@@ -13,6 +14,11 @@ from torch.autograd.function import once_differentiable
 
 from . import kernel_library as kl
 from . import ops
+
+
+def _no_tangent(*tensors: torch.Tensor) -> None:
+    if ops.has_tangent(*tensors):
+        raise NotImplementedError("the routing of tokens has no derivatives in forward mode, nor do its gradients")
 
 
 class _Dispatch(torch.autograd.Function):
@@ -26,6 +32,7 @@ class _Dispatch(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         (position,) = ctx.saved_tensors
+        _no_tangent(grad)
         return ops.route_combine(grad, position, None, ctx.dtype), None, None
 
 
@@ -39,6 +46,7 @@ class _Combine(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         rows, weights, position, offsets = ctx.saved_tensors
+        _no_tangent(grad)
         need_rows, need_weights = ctx.needs_input_grad[:2]
         return (*ops.route_combine_grad(grad, rows, position, offsets, weights, need_rows, need_weights), None, None, None)
 
@@ -69,6 +77,7 @@ class TokenRouting:
         rows = kl.host().route_dispatch(x, self.position, self.offsets) if x.dim() == 2 == self.position.dim() else None
         if rows is not None:
             return rows
+        _no_tangent(x)
         position = self._position2d()
         x2 = x.reshape(position.shape[0], x.shape[-1])
         if torch.is_grad_enabled() and x2.requires_grad:
@@ -86,6 +95,7 @@ class TokenRouting:
         out = kl.host().route_combine(rows, w, self.position, self.offsets, ops.elem_of(out_dtype))
         if out is not None:
             return out if weights.dim() == 2 else out.view(*weights.shape[:-1], rows.shape[-1])
+        _no_tangent(rows, w)
         position = self._position2d()
         w = w.view(position.shape)
         if torch.is_grad_enabled() and (rows.requires_grad or w.requires_grad):
