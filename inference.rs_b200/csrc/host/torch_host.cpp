@@ -669,6 +669,21 @@ Tensor grad_rows_of(const Tensor& g, int64_t& ld) {
 void no_tangent(const Tensor& grad) { TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(grad), "the routing of tokens has no derivatives in forward mode, nor do its gradients"); }
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
+// passes a gradient on that is not to be differentiated again
+struct OnceFunction : torch::autograd::Function<OnceFunction> {
+    static Tensor forward(AutogradContext*, const Tensor& grad) { return grad; }
+    static variable_list backward(AutogradContext*, variable_list) { TORCH_CHECK(false, "the gradients of token routing cannot be differentiated again"); }
+};
+// A gradient made of `sources`: under create_graph one that raises if it is differentiated, towards whichever of them.
+Tensor once(Tensor grad, std::initializer_list<const Tensor*> sources) {
+    if (!grad.defined() || !c10::GradMode::is_enabled()) return grad;
+    for (const Tensor* t : sources)
+        if (t->requires_grad()) {
+            grad.set_requires_grad(true);
+            return OnceFunction::apply(grad);
+        }
+    return grad;
+}
 struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& position, const Tensor& offsets) {
         ctx->save_for_backward({position});
@@ -679,11 +694,10 @@ struct DispatchFunction : torch::autograd::Function<DispatchFunction> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const Tensor position = ctx->get_saved_variables()[0];
-        TORCH_CHECK(!c10::GradMode::is_enabled(), "the gradient of dispatch cannot be differentiated again (create_graph)");
         no_tangent(grads[0]);
         int64_t ld;
         const Tensor g = grad_rows_of(grads[0], ld);
-        return {combine(g, ld, position, nullptr, (ScalarType)ctx->saved_data["type"].toInt()), Tensor(), Tensor()};
+        return {once(combine(g, ld, position, nullptr, (ScalarType)ctx->saved_data["type"].toInt()), {&grads[0]}), Tensor(), Tensor()};
     }
 };
 struct CombineFunction : torch::autograd::Function<CombineFunction> {
@@ -696,7 +710,6 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
         const Tensor &rows = saved[0], &weights = saved[1], &position = saved[2], &offsets = saved[3];
-        TORCH_CHECK(!c10::GradMode::is_enabled(), "the gradient of combine cannot be differentiated again (create_graph)");
         no_tangent(grads[0]);
         int64_t ldg, ldr;
         const Tensor g = grad_rows_of(grads[0], ldg);
@@ -710,7 +723,7 @@ struct CombineFunction : torch::autograd::Function<CombineFunction> {
                                        (int)offsets.numel() - 1, weights.data_ptr<float>(), grad_rows.defined() ? grad_rows.data_ptr() : nullptr,
                                        grad_weights.defined() ? grad_weights.data_ptr<float>() : nullptr, (int)tokens, (int)topk, (int)rows.size(1), on.stream),
                 "b200q_route_combine_grad");
-        return {grad_rows, grad_weights, Tensor(), Tensor(), Tensor()};
+        return {once(grad_rows, {&grads[0], &weights}), once(grad_weights, {&grads[0], &rows}), Tensor(), Tensor(), Tensor()};
     }
 };
 

@@ -10,7 +10,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import kernel_library as kl
 from . import ops
@@ -21,6 +20,25 @@ def _no_tangent(*tensors: torch.Tensor) -> None:
         raise NotImplementedError("the routing of tokens has no derivatives in forward mode, nor do its gradients")
 
 
+class _Once(torch.autograd.Function):
+    """Passes a gradient on that is not to be differentiated again."""
+
+    @staticmethod
+    def forward(ctx, grad):
+        return grad
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("the gradients of token routing cannot be differentiated again")
+
+
+def _once(grad: torch.Tensor | None, *sources: torch.Tensor) -> torch.Tensor | None:
+    """A gradient made of `sources`: under create_graph one that raises if it is differentiated, towards whichever of them."""
+    if grad is None or not torch.is_grad_enabled() or not any(t.requires_grad for t in sources):
+        return grad
+    return _Once.apply(grad.requires_grad_())
+
+
 class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, position, offsets):
@@ -29,11 +47,10 @@ class _Dispatch(torch.autograd.Function):
         return ops.route_dispatch(x, position, offsets)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
         (position,) = ctx.saved_tensors
         _no_tangent(grad)
-        return ops.route_combine(grad, position, None, ctx.dtype), None, None
+        return _once(ops.route_combine(grad, position, None, ctx.dtype), grad), None, None
 
 
 class _Combine(torch.autograd.Function):
@@ -43,12 +60,12 @@ class _Combine(torch.autograd.Function):
         return ops.route_combine(rows, position, weights, out_dtype)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
         rows, weights, position, offsets = ctx.saved_tensors
         _no_tangent(grad)
         need_rows, need_weights = ctx.needs_input_grad[:2]
-        return (*ops.route_combine_grad(grad, rows, position, offsets, weights, need_rows, need_weights), None, None, None)
+        grad_rows, grad_weights = ops.route_combine_grad(grad, rows, position, offsets, weights, need_rows, need_weights)
+        return _once(grad_rows, grad, weights), _once(grad_weights, grad, rows), None, None, None
 
 
 class TokenRouting:

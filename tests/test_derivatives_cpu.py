@@ -73,3 +73,24 @@ def test_tangents_of_gradients_are_refused(stubbed):
             grad = fwd.make_dual(torch.ones_like(out), torch.ones_like(out))
             with pytest.raises(NotImplementedError, match="forward mode"):
                 torch.autograd.grad(out, inputs, grad)
+
+
+def test_first_gradients_under_create_graph_and_no_second_ones(stubbed):
+    r = routing()
+    x, rows, w = torch.randn(3, 4, requires_grad=True), torch.randn(6, 4, requires_grad=True), torch.rand(3, 2, requires_grad=True)
+    for fn, inputs in ((lambda: r.dispatch(x), (x,)), (lambda: r.combine(rows, w), (rows, w))):
+        loss = lambda: (fn() ** 2).sum()
+        plain, first = torch.autograd.grad(loss(), inputs), torch.autograd.grad(loss(), inputs, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, first)) and all(g.requires_grad for g in first)
+        for g in first:
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                g.sum().backward(retain_graph=True)
+    # the output's own gradient is a constant here, but those of rows and weights depend on each other
+    first = torch.autograd.grad(r.combine(rows, w).sum(), (rows, w), create_graph=True)
+    for g in first:
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            g.sum().backward(retain_graph=True)
+    # and that of dispatch on nothing
+    assert not torch.autograd.grad(r.dispatch(x).sum(), x, create_graph=True)[0].requires_grad
+    only, = torch.autograd.grad(r.combine(rows, w.detach()).sum(), rows, create_graph=True)
+    assert not only.requires_grad

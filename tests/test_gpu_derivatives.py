@@ -71,3 +71,30 @@ def test_function_transforms_are_refused(state):
             torch.func.grad(lambda t: call(t).sum())(rows)
         with pytest.raises((RuntimeError, ValueError)):
             torch.func.jvp(call, (rows,), (rows,))
+
+
+def test_first_gradients_under_create_graph_and_no_second_ones(state):
+    r, _, x, rows, w, _, _ = state
+    for t in (x, rows, w):
+        t.requires_grad_()
+    for fn, inputs in ((lambda: r.dispatch(x), (x,)), (lambda: r.combine(rows, w), (rows, w)), (lambda: r.combine(rows.unsqueeze(1)[:, 0], w), (rows, w))):
+        loss = lambda: (fn() ** 2).sum()
+        plain, first = torch.autograd.grad(loss(), inputs), torch.autograd.grad(loss(), inputs, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, first)) and all(g.requires_grad for g in first)
+        for g in first:
+            with pytest.raises(RuntimeError, match="differentiated again"):
+                g.sum().backward(retain_graph=True)
+    # the output's own gradient is a constant here, but those of rows and weights depend on each other
+    first = torch.autograd.grad(r.combine(rows, w).sum(), (rows, w), create_graph=True)
+    for g in first:
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            g.sum().backward(retain_graph=True)
+    # and that of dispatch on nothing
+    assert not torch.autograd.grad(r.dispatch(x).sum(), x, create_graph=True)[0].requires_grad
+    only, = torch.autograd.grad(r.combine(rows, w.detach()).sum(), rows, create_graph=True)
+    assert not only.requires_grad
+    # inside a larger graph
+    v = torch.ones(64, device="cuda", requires_grad=True)
+    out = (r.combine(r.dispatch(x), w) * v).sum() + (v ** 3).sum()
+    gx, _ = torch.autograd.grad(out, (x, v), create_graph=True)
+    assert torch.equal(gx, torch.autograd.grad((r.combine(r.dispatch(x), w) * v).sum(), x)[0])
