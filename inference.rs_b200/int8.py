@@ -64,7 +64,8 @@ class Int8Tensor:
         """GGUF weights, quantized again with one scale per row: [n, k] of one matrix, [experts, n, k] of several."""
         if not weights or any(w.shape != weights[0].shape for w in weights):
             raise ValueError(f"expected matrices of one shape, got {[w.shape for w in weights]}")
-        parts = [ops.int8_quantize(w.dequantize(torch.float32)) for w in weights]
+        with torch.cuda.device(ops._one_device(*(w.data for w in weights))):  # QTensor launches on the current device
+            parts = [ops.int8_quantize(w.dequantize(torch.float32)) for w in weights]
         if len(parts) == 1:
             return cls._of_rows(*parts[0], weights[0].shape)
         return cls._of_rows(torch.cat([q for q, _ in parts]), torch.cat([s for _, s in parts]), (len(parts), *weights[0].shape))
