@@ -15,31 +15,24 @@ constexpr int INT8_MAX_EXPERTS = 1024;
 // Activation of a gated product, act(gate) * up, by the ids of the reference's host side
 // (crates/inference-quant/kernels/cuda/glu_activation.cuh:4-10); -1: the product is not gated.
 enum Int8Act : int { INT8_ACT_NONE = -1, INT8_ACT_SILU = 0, INT8_ACT_GELU = 1, INT8_ACT_RELU = 2, INT8_ACT_GELU_ERF = 3, INT8_ACT_SIGMOID = 4 };
-// One exponential and one reciprocal, each an instruction of its own right: off by some units of the last place, the exponential by as
-// many more as its argument has units (|x| 2^-23 relative, which x / (1 + exp(-x)) takes up by a quarter of x at most); results under the
-// smallest normal float are 0. With expf and an IEEE division the epilogue of 256 x 256 values took 54000 cycles where the product took
-// 16000.
-__device__ __forceinline__ float exp_fast(float x) {
+// x / (1 + exp(-t)) without a branch, its error in proportion to its size everywhere: exp(-|t|) neither overflows nor cancels, and the
+// reciprocal is one of 1 to 2. Two units of the last place for the exponential, one for the reciprocal, half of one for each other
+// rounding (for t below -87, where the exponential is subnormal, 2^-148 |x|). The layer of 2048 tokens through 2 of 8 experts of 4096 x
+// 14336 takes 708 us; 700 with ex2.approx of -t log2(e) and rcp.approx of 1 + exp(-t), which are off by |t| 2^-24 below zero and give 0
+// from -87 on; 720 with a Newton step on the reciprocal. With an IEEE division the epilogue is longer than the product.
+__device__ __forceinline__ float times_sigmoid(float x, float t) {
+    const float e = expf(-fabsf(t)), d = 1.0f + e;
     float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.4426950408889634f));
-    return r;
-}
-__device__ __forceinline__ float reciprocal_fast(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+    return (t < 0.0f ? x * e : x) * r;
 }
 __device__ __forceinline__ float int8_activate(float x, int act) {
     switch (act) {
-        case INT8_ACT_GELU: {
-            // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u))
-            const float u = 0.7978845608f * (x + 0.044715f * (x * x * x));
-            return x * reciprocal_fast(1.0f + exp_fast(-2.0f * u));
-        }
+        case INT8_ACT_GELU: return times_sigmoid(x, 1.5957691216f * (x + 0.044715f * (x * x * x)));  // 0.5 (1 + tanh u) = 1 / (1 + exp(-2 u))
         case INT8_ACT_RELU: return x > 0.0f ? x : (x <= 0.0f ? 0.0f : x);  // a NaN stays one
         case INT8_ACT_GELU_ERF: return 0.5f * x * (1.0f + erff(x * 0.70710678118654752440f));
-        case INT8_ACT_SIGMOID: return reciprocal_fast(1.0f + exp_fast(-x));
-        default: return x * reciprocal_fast(1.0f + exp_fast(-x));
+        case INT8_ACT_SIGMOID: return times_sigmoid(1.0f, x);
+        default: return times_sigmoid(x, x);
     }
 }
 
