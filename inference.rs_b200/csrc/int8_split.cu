@@ -8,6 +8,8 @@
 // (256 x 4096 x 4096 in tiles of 256 15.3). Parts through global memory instead, by whichever pair comes last, cost 4 us more.
 //
 // Every wait is bounded, as in int8_pair.cu; a CTA that gave up still comes to the cluster's barriers.
+#include <atomic>
+
 #include "int8_pair.cuh"
 
 namespace b200q {
@@ -203,12 +205,13 @@ __global__ void __cluster_dims__(2 * S, 1, 1) __launch_bounds__(I8P_THREADS, 1)
     if (warp == 2) tmem_dealloc_pair(tmem_base, I8S_TOKENS);
 }
 
-// How many clusters of the kernel the device holds at once.
+// How many clusters of the kernel the device holds at once; asked once per device, by whichever threads call first.
 template <auto kernel> static int clusters_at_once(int ctas, size_t smem) {
-    static int known[64];
+    static std::atomic<int> known[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-    if (known[dev] == 0) {
+    int n = known[dev].load();
+    if (n == 0) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)ctas, 1, 1);
         cfg.blockDim = dim3(I8P_THREADS, 1, 1);
@@ -219,14 +222,14 @@ template <auto kernel> static int clusters_at_once(int ctas, size_t smem) {
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        int n = 0;
         if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
             cudaGetLastError();
             n = 0;
         }
-        known[dev] = n > 0 ? n : -1;
+        n = n > 0 ? n : -1;
+        known[dev].store(n);
     }
-    return known[dev] > 0 ? known[dev] : 0;
+    return n > 0 ? n : 0;
 }
 
 template <typename OutT, int S> static int split_t(const Int8Product& p, int bn, cudaStream_t s, bool dependent) {
