@@ -539,7 +539,7 @@ PyObject* py_int8_forward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     long n, k;
     if (nargs != 5 || !int_args(args, {{2, &n}, {3, &k}})) return none();
     const Tensor *w = tensor_arg(args[0]), *ws = tensor_arg(args[1]), *x = tensor_arg(args[4]);
-    if (!of(w, ScalarType::Char) || !of(ws, ScalarType::Float) || !cuda_contiguous(x) || x->dim() < 2 || x->size(-1) != k || k < 1 || n < 1 || n > MOST || wants_grad(*x) || has_tangent(*x)) return none();
+    if (!of(w, ScalarType::Char) || !of(ws, ScalarType::Float) || !cuda_contiguous(x) || x->dim() < 2 || x->size(-1) != k || k < 1 || k > MOST || n < 1 || n > MOST || wants_grad(*x) || has_tangent(*x)) return none();
     const int64_t kp = pad(k, INT8_ROW_ALIGN), m = x->numel() / k;
     const int elem = elem_of(x->scalar_type());
     if (elem < 0 || m == 0 || m > MOST || w->dim() != 2 || w->size(0) != n || w->size(1) != kp || ws->numel() != n || !same_device(*x, {w, ws})) return none();
@@ -579,7 +579,7 @@ PyObject* py_int8_dequantize(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     ScalarType t;
     if (nargs != 4 || !int_args(args, {{2, &k}, {3, &elem}}) || !elem_scalar(elem, t)) return none();
     const Tensor *q = tensor_arg(args[0]), *scales = tensor_arg(args[1]);
-    if (!of(q, ScalarType::Char) || !of(scales, ScalarType::Float) || q->dim() < 2 || k < 1 || q->size(-1) != pad(k, INT8_ROW_ALIGN) || q->numel() == 0 || !same_device(*q, {scales})) return none();
+    if (!of(q, ScalarType::Char) || !of(scales, ScalarType::Float) || q->dim() < 2 || k < 1 || k > MOST || q->size(-1) != pad(k, INT8_ROW_ALIGN) || q->numel() == 0 || !same_device(*q, {scales})) return none();
     const int64_t rows = q->numel() / q->size(-1);
     if (scales->numel() != rows || rows > MOST) return none();
     OnDevice on(*q);
@@ -609,7 +609,7 @@ PyObject* py_int8_experts(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     for (int64_t i = 0; i + 1 < x.dim(); ++i)
         if (x.size(i) != ids.size(i)) return none();
     const int64_t hidden = x.size(-1), tokens = x.numel() / hidden, topk = ids.size(-1), experts = gate_up.size(0), p = pad(ffn, 8);
-    if (tokens * topk > MOST || gate_up.size(1) != 2 * p || gate_up.size(2) != pad(hidden, INT8_ROW_ALIGN) || down.size(0) != experts || down.size(1) != hidden ||
+    if (tokens * topk > MOST || hidden > MOST || ffn > MOST || experts > MOST || gate_up.size(1) != 2 * p || gate_up.size(2) != pad(hidden, INT8_ROW_ALIGN) || down.size(0) != experts || down.size(1) != hidden ||
         down.size(2) != pad(ffn, INT8_ROW_ALIGN) || gus.numel() != experts * 2 * p || ds.numel() != experts * hidden)
         return none();
     OnDevice on(x);

@@ -378,6 +378,12 @@ def _one_device(*tensors: torch.Tensor) -> torch.device:
     return tensors[0].device
 
 
+def _check_sizes(what: str, *sizes: int) -> None:
+    """The library takes sizes of 32 bits, and ctypes would cut larger ones down to them."""
+    if max(sizes, default=0) >= 1 << 31:
+        raise ValueError(f"{what}: a size of {max(sizes)} does not fit 32 bits")
+
+
 def has_tangent(*tensors: torch.Tensor) -> bool:
     """A derivative of forward mode comes with one of them: it is there without `requires_grad`, and under `no_grad` too."""
     return torch._C._is_fwd_grad_enabled() and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
@@ -413,6 +419,7 @@ def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     if done is not None:
         return done
     elem = elem_of(x.dtype)
+    _check_sizes("int8_quantize", *x.shape)
     dev = _one_device(x)
     x, ldx = _rows2d(x, "int8_quantize")
     m, k = x.shape
@@ -427,6 +434,7 @@ def int8_quantize(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def int8_dequantize(q: torch.Tensor, scales: torch.Tensor, k: int, out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """`b200q_int8_dequantize`: int8 rows and their scales -> the values [m, k] they stand for."""
     elem = elem_of(out_dtype)
+    _check_sizes("int8_dequantize", *q.shape, k)
     dev = _one_device(q, scales)
     _check_int8_rows(q, k, "int8 rows")
     _check_vector(scales, torch.float32, q.shape[0], "scales")
@@ -443,6 +451,7 @@ def int8_gemm(xq: torch.Tensor, x_scales: torch.Tensor, wq: torch.Tensor, w_scal
     w_scales [experts, n] and int32 offsets [experts + 1] rows offsets[e]..offsets[e + 1] meet matrix e; the rows behind the last
     expert's are not written."""
     elem = elem_of(out_dtype)
+    _check_sizes("int8_gemm", *xq.shape, *wq.shape, k)
     dev = _one_device(xq, x_scales, wq, w_scales, *(t for t in (offsets, out) if t is not None))
     experts = wq.shape[0] if wq.dim() == 3 else 1
     n = wq.shape[-2]
@@ -468,6 +477,7 @@ def int8_matmul(x: torch.Tensor, wq: torch.Tensor, w_scales: torch.Tensor) -> to
     """`b200q_int8_matmul`: x [m, k] (f32, f16 or bf16; rows may be strided) becomes int8 rows, times wq [n, kp] -> [m, n] of x's
     type."""
     elem = elem_of(x.dtype)
+    _check_sizes("int8_matmul", *x.shape, *wq.shape)
     dev = _one_device(x, wq, w_scales)
     x, ldx = _rows2d(x, "int8_matmul")
     m, k = x.shape
@@ -490,6 +500,7 @@ def route_sort(ids: torch.Tensor, experts: int) -> tuple[torch.Tensor, torch.Ten
     offsets[e]..offsets[e + 1], slot s is row position[s] (-1: none)."""
     if ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"expert ids must be int32 or int64, not {ids.dtype}")
+    _check_sizes("route_sort", ids.numel(), experts)
     dev = _one_device(ids)
     ids = ids.contiguous()
     order = torch.empty(ids.numel(), dtype=torch.int32, device=dev)
@@ -511,6 +522,7 @@ def _check_position(position: torch.Tensor, tokens: int | None = None) -> None:
 def route_dispatch(x: torch.Tensor, position: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
     """`b200q_route_dispatch`: x [tokens, h] -> rows [tokens * slots, h] in the order of the experts; rows behind the last are zeros."""
     elem = elem_of(x.dtype)
+    _check_sizes("route_dispatch", *x.shape, position.numel(), offsets.numel())
     dev = _one_device(x, position, offsets)
     x, ldx = _rows2d(x, "route_dispatch")
     tokens, h = x.shape
@@ -528,6 +540,7 @@ def route_combine(rows: torch.Tensor, position: torch.Tensor, weights: torch.Ten
     """`b200q_route_combine`: rows [tokens * slots, h] back to [tokens, h], each token the sum of its rows times its weights (f32
     [tokens, slots]; None: 1 each), in f32 and in slot order."""
     elem_in, elem_out = elem_of(rows.dtype), elem_of(out_dtype)
+    _check_sizes("route_combine", *rows.shape, position.numel())
     dev = _one_device(rows, position, *(() if weights is None else (weights,)))
     rows, ldr = _rows2d(rows, "route_combine")
     _check_position(position)
@@ -548,6 +561,7 @@ def route_combine_grad(grad_out: torch.Tensor, rows: torch.Tensor, position: tor
                        need_rows: bool = True, need_weights: bool = True) -> tuple[torch.Tensor | None, torch.Tensor | None]:
     """`b200q_route_combine_grad`: the gradients of `route_combine` towards its rows (in their type) and its weights (f32)."""
     elem_g, elem = elem_of(grad_out.dtype), elem_of(rows.dtype)
+    _check_sizes("route_combine_grad", *grad_out.shape, *rows.shape, position.numel(), offsets.numel())
     dev = _one_device(grad_out, rows, position, offsets, weights)
     grad_out, ldg = _rows2d(grad_out, "route_combine_grad")
     rows, ldr = _rows2d(rows, "route_combine_grad")
@@ -573,6 +587,7 @@ def int8_experts(x: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor, gate
     """`b200q_int8_experts`: x [tokens, h] through the experts that ids [tokens, slots] names, weighted (f32). gate_up as
     `Int8Experts` lays it out."""
     elem = elem_of(x.dtype)
+    _check_sizes("int8_experts", *x.shape, ids.numel(), *gate_up.shape, *down.shape, ffn)
     dev = _one_device(x, ids, weights, gate_up, gate_up_scales, down, down_scales)
     x, ldx = _rows2d(x, "int8_experts")
     tokens, hidden = x.shape
