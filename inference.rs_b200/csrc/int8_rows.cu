@@ -14,6 +14,7 @@ namespace b200q {
 
 constexpr int I8R_WARPS = 8;
 constexpr int I8R_STEP = 64;  // k of one piece
+constexpr int I8R_PER_SM = 2; // CTAs on an SM
 
 __device__ __forceinline__ uint4 ldg_stream(const int8_t* p) {
     uint4 v;
@@ -58,8 +59,8 @@ template <int R, int NT, int U, int WK> struct RowPieces {
     }
 };
 
-template <typename OutT, int R, int NT, int U, int WK, int PER_SM>
-__global__ void __launch_bounds__(32 * I8R_WARPS, PER_SM) int8_rows_kernel(const Int8Product p) {
+template <typename OutT, int R, int NT, int U, int WK>
+__global__ void __launch_bounds__(32 * I8R_WARPS, I8R_PER_SM) int8_rows_kernel(const Int8Product p) {
     constexpr int ROWS = 16 * R, TOKENS = 8 * NT, PITCH = ROWS + 4, GROUPS = I8R_WARPS / WK;
     __shared__ int sums[I8R_WARPS][TOKENS][PITCH];
     extern __shared__ int lists[];
@@ -155,42 +156,50 @@ __global__ void __launch_bounds__(32 * I8R_WARPS, PER_SM) int8_rows_kernel(const
     }
 }
 
-template <typename OutT, int R, int NT, int U, int WK, int PER_SM> static cudaError_t rows_launch(const Int8Product& p, cudaStream_t s, bool dependent) {
+template <typename OutT, int R, int NT, int U, int WK> static cudaError_t rows_launch(const Int8Product& p, cudaStream_t s, bool dependent) {
     // at most one group of tokens more per expert than the rows fill
-    const long long tiles = (long long)((p.n + 16 * R - 1) / (16 * R)) * ((p.rows + 8 * NT - 1) / (8 * NT) + p.experts - 1), fit = (long long)PER_SM * runtime_info().sm_count;
-    return launch_kernel(int8_rows_kernel<OutT, R, NT, U, WK, PER_SM>, dim3((unsigned)(tiles < fit ? tiles : fit), 1, 1), 32 * I8R_WARPS, int8_list_bytes(p.experts), s, dependent, p);
+    const long long tiles = (long long)((p.n + 16 * R - 1) / (16 * R)) * ((p.rows + 8 * NT - 1) / (8 * NT) + p.experts - 1), fit = (long long)I8R_PER_SM * runtime_info().sm_count;
+    return launch_kernel(int8_rows_kernel<OutT, R, NT, U, WK>, dim3((unsigned)(tiles < fit ? tiles : fit), 1, 1), 32 * I8R_WARPS, int8_list_bytes(p.experts), s, dependent, p);
 }
 // Which form of the kernel takes a product; none where the tensor-core kernels (int8_pair.cu, int8_split.cu) are the faster ones. What
-// decides is how many 16-row tiles there are for 2368 warps, and how many tokens meet each weight. us, quantizer included, bf16, weights
-// out of HBM (tc: the tensor-core kernels):
-//   up to 8 tokens   8 warps a tile: 4096 x 1024 4.5 (4: 5.5, tc 8.2), 4096 x 4096 6.4 (4: 7.0), 14336 x 4096 13.5 (4: 16.5, tc 17.1)
-//                    4 warps:        one token through 2 of 8 experts of 4096 x 14336 68.9 (8: 72.7)
-//                    2 warps and 32 rows: 4096 x 28672 21.8 (4: 22.6, tc 24.3); 16 tokens through 8 of 128 experts of 2048 x 768 67.8
-//                    (4 warps, 16 rows: 78.2, tc 73.5). Experts with five tokens and more: tc (48 tokens through 6 of 64: 97.8, 98.5)
-//   more, 16 at once 16 rows:        16 tokens 4096 x 4096 7.3 (tc 10.1), 14336 x 4096 15.6 (17.2); 64 tokens 4096 x 1024 6.4 (8.3)
-//                    32 rows:        32 tokens 4096 x 4096 8.9 (16 rows 9.7, tc 10.2)
-//                    none, by groups of 16 tokens x tiles: 16 tokens 4096 x 14336 16.5 (tc 15.2), 48 tokens 4096 x 4096 13.1 (10.7), 96
-//                    tokens 4096 x 2048 13.4 (9.9); long rows sooner: 32 tokens 8192 x 4096 14.0 (12.5), 14336 x 4096 21.3 (17.3)
+// decides is how the tiles of 16 rows fill the places that the SMs have for CTAs (two each, 296 on 148), and how many tokens meet each
+// weight: a tile more than the places are, and some SM has twice the work. us, quantizer included, bf16, weights out of HBM (tc: the
+// tensor-core kernels):
+//   up to 8 tokens   8 warps a tile while every tile has a place, then 4 (two tiles a CTA): of 14336 k 296 tiles 14.0 (4: 16.5), 304 18.0
+//                    (16.8), 448 20.2 (19.5); of 4096 k 6.2 (6.9), 7.7 (7.1), 8.3 (8.1); of 1024 k 3.9 (3.9), 4.5 (3.9), 4.9 (4.3). 4 warps
+//                    up to four tiles a place, then 2 warps and 32 rows: of 14336 k 1184 tiles 42.9 (2: 47.0), 1200 48.7 (47.3), 1792
+//                    68.7 (64.5); of 4096 k 14.9 (17.0), 16.4 (17.1), 21.7 (21.1); of 1024 k 6.6 (6.5), 7.1 (6.7), 9.0 (7.9)
+//                    experts: one token through 2 of 8 of 4096 x 14336, 4 warps for the 512 tiles of down 68.9 (8: 72.7); 16 tokens through
+//                    8 of 128 of 2048 x 768 67.8 with 2 (4 warps 78.2, tc 73.5). Experts with five to eight tokens, of which some have
+//                    more: 4 warps up to six tiles a place, then tc (20 tokens through 1 of 4 of 1024 x 2400, 1200 tiles, 17.2 and 19.2; 10
+//                    through 2 of 4 of 4096 x 3500, 1752 tiles, 41 and 61, but 24 through 4 of 16 of 2048 x 800, 1600 tiles, 30.9 and 28.8;
+//                    48 through 6 of 64 of 2048 x 1408, 11264 tiles, 98.5 and 97.8)
+//   more, 16 at once a group is 16 tokens of a tile. Of long rows as many groups as places: 16 tokens of 14336 k 288 groups 15.6 (tc
+//                    17.6), 320 23.9 (18.6); of 8192 k 11.1 (13.3), 15.8 (13.9). Of rows up to 6144 twice as many: of 6144 k 288 9.1 (11.7),
+//                    320 12.7 (12.2), 513 14.2 (14.5), 640 18.1 (16.6); of 4096 k 513 10.7 (12.2), 640 13.4 (13.2)
+//                    with more groups than places and more than 16 tokens, 32 rows a tile: 32 tokens of 4096 k 512 groups 8.6 (16 rows 9.7,
+//                    tc 10.1), 640 13.2 (tc 10.7)
 enum class RowsForm { none, few_tiles, some_tiles, many_tiles, tokens16, tokens32 };
 static RowsForm rows_form(const Int8Product& p) {
     const int used = p.experts < p.rows ? p.experts : p.rows;  // experts with tokens, at most
     const int per = (p.rows + used - 1) / used;
     const long long tiles = (long long)((p.n + 15) / 16) * used;
-    if (per <= 8 && tiles < 1536) return tiles < 512 ? RowsForm::few_tiles : RowsForm::some_tiles;
+    const long long places = (long long)I8R_PER_SM * runtime_info().sm_count;
+    if (per <= 8 && tiles <= (p.experts > 1 && per > 4 ? 6 : 4) * places) return tiles <= places ? RowsForm::few_tiles : RowsForm::some_tiles;
     if (per <= (p.experts > 1 ? 4 : 8)) return RowsForm::many_tiles;
     const long long groups = (per + 15) / 16 * tiles;
-    if (groups <= (p.k > 6144 ? 256 : 512)) return groups <= 256 || per <= 16 ? RowsForm::tokens16 : RowsForm::tokens32;
+    if (groups <= (p.k > 6144 ? places : 2 * places)) return groups <= places || per <= 16 ? RowsForm::tokens16 : RowsForm::tokens32;
     return RowsForm::none;
 }
 bool int8_rows_pays(const Int8Product& p) { return rows_form(p) != RowsForm::none; }
 
 template <typename OutT> static cudaError_t rows_t(const Int8Product& p, cudaStream_t s, bool dependent) {
     switch (rows_form(p)) {
-        case RowsForm::few_tiles: return rows_launch<OutT, 1, 1, 4, 8, 2>(p, s, dependent);
-        case RowsForm::some_tiles: return rows_launch<OutT, 1, 1, 4, 4, 2>(p, s, dependent);
-        case RowsForm::many_tiles: return rows_launch<OutT, 2, 1, 2, 2, 2>(p, s, dependent);
-        case RowsForm::tokens16: return rows_launch<OutT, 1, 2, 2, 8, 2>(p, s, dependent);
-        default: return rows_launch<OutT, 2, 2, 1, 8, 2>(p, s, dependent);
+        case RowsForm::few_tiles: return rows_launch<OutT, 1, 1, 4, 8>(p, s, dependent);
+        case RowsForm::some_tiles: return rows_launch<OutT, 1, 1, 4, 4>(p, s, dependent);
+        case RowsForm::many_tiles: return rows_launch<OutT, 2, 1, 2, 2>(p, s, dependent);
+        case RowsForm::tokens16: return rows_launch<OutT, 1, 2, 2, 8>(p, s, dependent);
+        default: return rows_launch<OutT, 2, 2, 1, 8>(p, s, dependent);
     }
 }
 
